@@ -130,7 +130,7 @@ int lumina_gemv_noalloc(const lumina_weight* w, const float* x_dev, int batch, i
  * peers (the decode GEMVs, the tcgen05 multi-row projection, the
  * tensor-parallel exchange) bound every wait; one that gives up ORs a bit
  * into a per-device fault word (1: gemv_fused, 2: gemv_tc, 4: peer exchange,
- * 8: gemm_tc05) and returns, leaving its outputs unwritten. Every
+ * 8: gemm_tc05, 16: gemv_tcb, 32: lumina_kvq_attend) and returns, leaving its outputs unwritten. Every
  * synchronous entry (lumina_gemv_host, lumina_forward, lumina_layer_forward,
  * lumina_decode_step, lumina_decode_greedy, lumina_profile_gemv) clears the
  * word as it starts and returns LUMINA_E_CUDA ("a device wait timed out")
@@ -301,6 +301,138 @@ int lumina_profile_gemv(lumina_model* m, int iters, float* ms_per_launch, int* l
  * and its algorithmic bytes (the K and V rows of every cached key of this
  * shard's heads, q in, the output out). Leaves the KV rows unchanged. */
 int lumina_profile_attention(lumina_model* m, int iters, float* ms_per_launch, double* bytes_per_launch);
+
+/* ---- serving several sequences: quantized KV pages, logits ------------ */
+/* No reference counterpart (the reference decodes one sequence, its cache is
+ * float, chat.py:418-551). What one step of several requests does around
+ * the packed projections: write the new rows' K and V into quantized pages,
+ * attend over them, hand rows back, and shape the logits. Every buffer is
+ * the caller's; the calls are asynchronous on `stream`, allocate nothing and
+ * can be captured into a CUDA graph. */
+
+/* Element type of activation rows (q, k, v, attention outputs). */
+enum { LUMINA_T_F32 = 0, LUMINA_T_F16 = 1 };
+
+/* A pool of KV pages: n_pages x n_kv blocks of lumina_kvq_block_bytes each.
+ * The block of (page p, KV head h) starts at pool_dev + (p * n_kv + h) *
+ * block_bytes and holds page_size tokens:
+ *   K codes  page_size x head_dim x bits / 8   (token-major)
+ *   V codes  page_size x head_dim x bits / 8
+ *   K scales page_size float32, V scales page_size float32
+ * bits 8: signed bytes -127..127, value = code * scale, scale = amax / 127.
+ * bits 4: codes 0..15 (even column in the low nibble, as in a .lumina file),
+ *   value = (2 code - 15) * scale, scale = amax / 15: the levels
+ *   linspace(-1, 1, 16) * amax of Lumina int4 (adapters/lumina.py:135-139).
+ * amax is over the token's head_dim values of that head. A row below 2^-100
+ * everywhere is stored as zero scale; a row with an infinity or a NaN gets a
+ * NaN scale, so what sees that key (and only that) becomes NaN. */
+typedef struct {
+  void* pool_dev;  /* 16-byte aligned */
+  int device;
+  int bits;        /* 8 or 4 */
+  int n_pages, n_kv;
+  int head_dim;    /* 64 or 128 */
+  int page_size;   /* 16, 32, 64 or 128 tokens */
+} lumina_kvq_pool;
+
+/* The sequences of one step. Sequence s owns rows [row_start[s],
+ * row_start[s+1]) of the activation matrices; they are its last rows, at
+ * positions len[s] - n .. len[s] - 1 (len counts the new rows). Token t of
+ * it lives in page pages[s * pages_ld + t / page_size]. n_rows =
+ * row_start[n_seq]; max_rows is at least every sequence's row count; a
+ * sequence may have no rows. The kernels check these device values: a row,
+ * length or page number out of range sets bit 64 of the device fault word
+ * (lumina_fault_status) and the affected rows are skipped. */
+typedef struct {
+  const int* row_start_dev; /* n_seq + 1 */
+  const int* len_dev;       /* n_seq */
+  const int* pages_dev;     /* n_seq x pages_ld */
+  int pages_ld;
+  int n_seq;                /* 1..4096 */
+  int n_rows, max_rows;
+} lumina_kvq_batch;
+
+int lumina_kvq_block_bytes(int bits, int head_dim, int page_size, size_t* bytes);
+
+/* Write the batch's new rows: q (n_rows, n_heads, head_dim), k and v
+ * (n_rows, n_kv, head_dim), rows ldq / ldk / ldv elements apart (so they may
+ * be column ranges of one fused projection). q and k: optional RMSNorm over
+ * each head with weights q_norm / k_norm (head_dim float32, NULL = none),
+ * x * (1 / sqrt(mean(x^2) + eps)) * w, then rotate-half RoPE (chat.py:88-103)
+ * with row `position` of the tables cos / sin (n_pos x head_dim / 2 float32);
+ * positions from n_pos on are out of range. q goes to q_out (rows ldqo
+ * apart, same type), k and v into the pool. Arithmetic in fp32, products
+ * rounded separately; codes round to nearest, ties to even. 16-byte aligned
+ * rows of every operand. */
+int lumina_kvq_append(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch, const void* q_dev, int ldq,
+                      const void* k_dev, int ldk, const void* v_dev, int ldv, int type, int n_heads,
+                      const float* q_norm_dev, const float* k_norm_dev, float eps, const float* cos_dev,
+                      const float* sin_dev, int n_pos, void* q_out_dev, int ldqo, void* stream);
+
+/* The values the pool holds for the batch's rows: K to k_out, V to v_out
+ * (n_rows, n_kv, head_dim), rows ldo elements apart, rounded once to `type`.
+ * A batch whose sequences "own" len[s] rows reads them whole. */
+int lumina_kvq_read(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch, void* k_out_dev, void* v_out_dev,
+                    int ldo, int type, void* stream);
+
+/* Attention of the batch's rows over their sequences' pages. Row i of
+ * sequence s sits at position p = len - n + i and sees key j < len iff
+ * (j <= p and (window == 0 or j > p - window)) or j < prefix[s].
+ *   x_j = scale * (q . k_j);  softcap > 0: x_j = softcap * tanh(x_j / softcap)
+ *   slopes: x_j -= slopes[head] * |p - j|
+ *   out = sum_j softmax(x)_j v_j, zero for a row that sees nothing.
+ * n_heads is a multiple of the pool's n_kv; query head h reads KV head
+ * h / (n_heads / n_kv). q and out rows are ldq / ldo elements apart, in
+ * `type`; scores, softmax statistics and sums are fp32. workspace_dev: at
+ * least lumina_kvq_workspace_bytes, zeroed once by the caller before its
+ * first use and left reusable by every call; calls that may overlap on the
+ * GPU need workspaces of their own. */
+typedef struct {
+  const void* q_dev;
+  void* out_dev;
+  int ldq, ldo;
+  int type;
+  int n_heads;
+  float scale;             /* 0: 1 / sqrt(head_dim) */
+  float softcap;           /* 0: none */
+  const float* slopes_dev; /* n_heads, or NULL */
+  const int* prefix_dev;   /* n_seq, or NULL */
+  int window;              /* 0: unlimited */
+  void* workspace_dev;
+  size_t workspace_bytes;
+} lumina_kvq_attend_args;
+int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch, const lumina_kvq_attend_args* args,
+                      void* stream);
+int lumina_kvq_workspace_bytes(int device, size_t* bytes);
+
+/* Shape logits rows (rows x vocab float32, ld elements apart) into out (may
+ * be the input): for every token t that occurs c > 0 times in the row's
+ * history, l = l > 0 ? l / repeat : l * repeat (the sampler's rule,
+ * chat.py:330-338), then l = l - frequency * c - presence; then l += bias of
+ * the row's (token, value) list (a token listed twice takes its last entry);
+ * then -inf where the row's grammar bit (bit t % 32 of word t / 32) is 0.
+ * Any part may be NULL. Tokens outside [0, vocab) are ignored. argmax gets
+ * the first index of the largest value (a NaN counts as largest, as in
+ * np.argmax; -1 never occurs: a row of all -inf gives 0). */
+typedef struct {
+  const float* logits_dev;
+  float* out_dev;
+  int ld, ldo;
+  int rows, vocab;
+  const int* hist_start_dev;  /* rows + 1 offsets into hist_tok, or NULL */
+  const int* hist_tok_dev;
+  const float* repeat_dev;    /* rows, > 0, or NULL (1) */
+  const float* frequency_dev; /* rows, or NULL (0) */
+  const float* presence_dev;  /* rows, or NULL (0) */
+  const int* bias_start_dev;  /* rows + 1 offsets, or NULL */
+  const int* bias_tok_dev;
+  const float* bias_val_dev;
+  const uint32_t* mask_dev;   /* rows x mask_ld words, or NULL */
+  int mask_ld;
+  int* argmax_dev;            /* rows, or NULL */
+  int device;
+} lumina_logits_args;
+int lumina_logits_adjust(const lumina_logits_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,132 @@
+// Warp-level pieces of the attention over quantized KV pages on mma.sync
+// m16n8k16: 16 query rows x 16 keys per step, codes straight from memory to
+// fragments.
+//
+// A warp step scores 16 packed query rows (row r = local row r / G, head r %
+// G of one KV head's G query heads) against 16 keys. Codes are small
+// integers, exact in fp16, so K and V enter the tensor pipe as they are
+// stored and the scales stay outside the products: a key's K scale
+// multiplies its score column, its V scale multiplies its probability.
+//
+// Fragment layouts (lane = 4 g + t): in the K fragment of key g, a thread's
+// four k-indices of a step are any four dims as long as q uses the same, so
+// thread t owns runs of the key's codes that load as 16-byte words
+// (dim_of). In the V fragment, n-tile i takes dim g * HD / 8 + i at column
+// g, so a thread loads one contiguous run per key and ends with the 2 HD / 8
+// contiguous output dims from 2 t HD / 8 on.
+#pragma once
+#include "kvq.cuh"
+
+namespace lumina {
+
+constexpr float KVQ_LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e as a float, e in [-126, 127]
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+// (a, b) -> fp16 pair, and the fp16 pair of what it leaves
+__device__ __forceinline__ uint32_t split_h2(float a, float b, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  lo = half2_bits(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+  return half2_bits(h);
+}
+
+// Codes to fp16 through the fp16 number 1024 + u: its low mantissa bits are u.
+constexpr uint32_t H_1024 = 0x64006400u;
+// signed bytes with the sign bit flipped (u = c + 128): two of them -> (c0, c1)
+template <int SEL>
+__device__ __forceinline__ uint32_t s8_pair(uint32_t flipped) {
+  const __half2 v = bits_half2(__byte_perm(flipped, 0x64646464u, SEL));
+  return half2_bits(__hsub2(v, __floats2half2_rn(1152.f, 1152.f)));
+}
+// nibbles at bits 4-7 of each 16-bit half -> 2 c - 15 = (1024 + 16 c) / 8 - 143
+// (at bits 0-3 the subtrahend, 2063, would not be an fp16 number)
+__device__ __forceinline__ uint32_t u4_pair(uint32_t w) {
+  return half2_bits(__hfma2(bits_half2((w & 0x00F000F0u) | H_1024), __floats2half2_rn(0.125f, 0.125f),
+                            __floats2half2_rn(-143.f, -143.f)));
+}
+
+template <int HD, int BITS>
+struct KvqFrag {
+  static constexpr int NB = HD * BITS / 8;  // code bytes of one key
+  static constexpr int KK = HD / 16;        // MMA steps of q . k
+  static constexpr int KW = NB / 16;        // 32-bit words of K codes per thread and key
+  static constexpr int NT = HD / 8;         // n-tiles of p . v = dims per thread and key
+  static constexpr int VW = NT * BITS / 32; // 32-bit words of V codes per thread and key
+
+  // dim of k-index e (0..3) of step kk for thread t
+  __device__ static __forceinline__ int dim_of(int t, int kk, int e) {
+    if constexpr (BITS == 8) return ((kk >> 2) * 4 + t) * 16 + (kk & 3) * 4 + e;
+    else return t * (HD / 4) + (kk >> 1) * 8 + 2 * (kk & 1) + (e >> 1) + 4 * (e & 1);
+  }
+  // the thread's K code words of one key row
+  __device__ static __forceinline__ void load_k(const uint8_t* row, int t, uint32_t (&w)[KW]) {
+    if constexpr (KW >= 4) {
+#pragma unroll
+      for (int i = 0; i < KW / 4; ++i) {
+        const uint4 q = *reinterpret_cast<const uint4*>(row + (i * 4 + t) * 16);
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(row + t * 8);
+      w[0] = q.x; w[1] = q.y;
+    }
+  }
+  // B fragment of step kk
+  template <int kk>
+  __device__ static __forceinline__ void k_frag(const uint32_t (&w)[KW], uint32_t& b0, uint32_t& b1) {
+    if constexpr (BITS == 8) {
+      const uint32_t f = w[kk] ^ 0x80808080u;
+      b0 = s8_pair<0x4140>(f);
+      b1 = s8_pair<0x4342>(f);
+    } else {
+      const uint32_t v = w[kk >> 1];
+      b0 = u4_pair((kk & 1) ? v >> 4 : v << 4);
+      b1 = u4_pair((kk & 1) ? v >> 8 : v);
+    }
+  }
+  __device__ static __forceinline__ void load_v(const uint8_t* row, int g, uint32_t (&w)[VW]) {
+    if constexpr (VW == 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(row + g * 16);
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    } else if constexpr (VW == 2) {
+      const uint2 q = *reinterpret_cast<const uint2*>(row + g * 8);
+      w[0] = q.x; w[1] = q.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(row + g * 4);
+    }
+  }
+  // fp16 pairs (key a, key b) of dims DPW * j + i of the thread's run, where
+  // word j of each key holds DPW = 32 / BITS dims
+  template <int i>
+  __device__ static __forceinline__ uint32_t v_pair(uint32_t a, uint32_t b) {
+    if constexpr (BITS == 8) {
+      // bytes (a_i, b_i) with 0x64 above each
+      const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7362 : 0x5140);  // a_i' b_i' a_i'+1 b_i'+1
+      return s8_pair<(i & 1) ? 0x4342 : 0x4140>(x ^ 0x80808080u);
+    } else {
+      const uint32_t x = __byte_perm(a, b, (i & 4) ? 0x7632 : 0x5410);
+      return u4_pair((i & 3) == 0 ? x << 4 : x >> (4 * ((i & 3) - 1)));
+    }
+  }
+};
+
+}  // namespace lumina

@@ -205,9 +205,10 @@ int clear_fault_async(cudaStream_t s) {
 }
 
 int fault_error(const char* what, int word) {
-  set_error("%s: a device wait timed out (fault word %#x:%s%s%s%s%s)", what, word,
+  set_error("%s: a device wait timed out (fault word %#x:%s%s%s%s%s%s%s)", what, word,
             (word & 1) ? " gemv_fused_kernel" : "", (word & 2) ? " gemv_tc_kernel" : "",
-            (word & 4) ? " peer exchange" : "", (word & 8) ? " gemm_tc05_kernel" : "", (word & 16) ? " gemv_tcb_kernel" : "");
+            (word & 4) ? " peer exchange" : "", (word & 8) ? " gemm_tc05_kernel" : "", (word & 16) ? " gemv_tcb_kernel" : "",
+            (word & 32) ? " lumina_kvq_attend" : "", (word & 64) ? " lumina_kvq batch out of range" : "");
   return LUMINA_E_CUDA;
 }
 

@@ -103,6 +103,13 @@ SIGNATURES = {
     "lumina_profile_attention": [_VP, _I, _FP, ctypes.POINTER(ctypes.c_double)],
     "lumina_fault_status": [_I, _IP, _I],
     "lumina_debug_wait_limit": [ctypes.c_longlong],
+    "lumina_kvq_block_bytes": [_I, _I, _I, ctypes.POINTER(_SZ)],
+    "lumina_kvq_append": [_VP, _VP, _VP, _I, _VP, _I, _VP, _I, _I, _I, _VP, _VP, ctypes.c_float, _VP, _VP, _I, _VP, _I,
+                          _VP],
+    "lumina_kvq_read": [_VP, _VP, _VP, _VP, _I, _I, _VP],
+    "lumina_kvq_attend": [_VP, _VP, _VP, _VP],
+    "lumina_kvq_workspace_bytes": [_I, ctypes.POINTER(_SZ)],
+    "lumina_logits_adjust": [_VP, _VP],
 }
 _RESTYPE = {"lumina_last_error": ctypes.c_char_p}
 
