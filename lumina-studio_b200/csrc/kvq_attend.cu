@@ -12,36 +12,14 @@
 #include <cfloat>
 #include <cmath>
 
+#include "kvq_attend.cuh"
 #include "kvq_mma.cuh"
 
 namespace lumina {
 
 namespace {
 
-struct AttendArgs {
-  KvqView v;
-  const void* q;
-  void* out;
-  size_t ldq, ldo;
-  int nh, G;
-  float scale, cap;
-  const float* slopes;
-  const int* prefix;
-  int window;
-};
-
 constexpr int AT_THREADS = 128;
-
-// rows of sequence s as the batch says (0 where row_start is out of order)
-__device__ __forceinline__ int seq_rows(const KvqView& v, int s, int& first) {
-  first = __ldg(v.row_start + s);
-  const int end = __ldg(v.row_start + s + 1);
-  if (first < 0 || end < first || end > v.n_rows || end - first > v.max_rows) {
-    kvq_fault(v, KVQ_FAULT_DATA);
-    return 0;
-  }
-  return end - first;
-}
 
 template <int HD, int BITS, typename T>
 __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
@@ -63,7 +41,10 @@ __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
   for (int s0 = 0; s0 < v.n_seq; s0 += AT_THREADS) {
     const int s = s0 + tid;
     int first, nb = 0;
-    if (s < v.n_seq) nb = (seq_rows(v, s, first) * a.G + 15) >> 4;
+    if (s < v.n_seq) {
+      const int n = kvq_seq_rows(v, s, first);
+      if (n * a.G > a.few) nb = (n * a.G + 15) >> 4;
+    }
     int inc = nb;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -87,7 +68,7 @@ __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
   if (s < 0) return;
   const int kvh = blockIdx.y;
   int first;
-  const int n = seq_rows(v, s, first);
+  const int n = kvq_seq_rows(v, s, first);
   const int cap_tokens = v.pages_ld << v.page_shift;
   int len = __ldg(v.len + s);
   if (len < 0 || len > cap_tokens) {
@@ -324,7 +305,17 @@ __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
 }
 
 template <int HD, int BITS, typename T>
-int attend_launch(const AttendArgs& a, cudaStream_t s) {
+int attend_launch(AttendArgs a, cudaStream_t s) {
+  // Sequences of few packed rows go to the decode kernel, the others here. A
+  // batch of equal row counts needs one of the two only.
+  const long long max_packed = (long long)a.v.max_rows * a.G;
+  a.few = max_packed <= KVQ_DECODE_ROWS ? KVQ_DECODE_ROWS : a.G <= 8 ? 8 : KVQ_DECODE_ROWS;
+  const bool equal = (long long)a.v.max_rows * a.v.n_seq == a.v.n_rows;
+  if (max_packed <= a.few || !equal) {
+    const int rc = kvq_decode_launch<HD, BITS, T>(a, (int)min(max_packed, (long long)a.few), s);
+    if (rc) return rc;
+  }
+  if (max_packed <= a.few) return LUMINA_OK;
   const long long blocks = ((long long)a.v.n_rows * a.G + 15) / 16 + a.v.n_seq;
   const dim3 grid((unsigned)blocks, a.v.n_kv);
   kvq_attend_kernel<HD, BITS, T><<<grid, AT_THREADS, 0, s>>>(a);
@@ -342,7 +333,7 @@ extern "C" {
 int lumina_kvq_workspace_bytes(int device, size_t* bytes) {
   LUMINA_CHECK_ARG(bytes, "kvq_workspace_bytes: null output");
   LUMINA_CHECK_ARG(device >= 0, "kvq_workspace_bytes: device %d", device);
-  *bytes = 1 << 20;
+  *bytes = kvq_ws_bytes();
   return LUMINA_OK;
 }
 
@@ -382,6 +373,10 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
   a.slopes = args->slopes_dev;
   a.prefix = args->prefix_dev;
   a.window = args->window;
+  a.min_cells = 16;
+  a.tickets = static_cast<int*>(args->workspace_dev);
+  a.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(args->workspace_dev) + KVQ_WS_TICKETS);
+  a.spin = wait_spin_limit();
   cudaStream_t s = (cudaStream_t)stream;
   const bool f16 = args->type == LUMINA_T_F16;
   if (hd == 128 && pool->bits == 8) return f16 ? attend_launch<128, 8, __half>(a, s) : attend_launch<128, 8, float>(a, s);

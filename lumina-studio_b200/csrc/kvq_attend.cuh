@@ -1,0 +1,69 @@
+// What the attention kernels over quantized KV pages share: arguments and
+// the launches that lumina_kvq_attend chooses from.
+#pragma once
+#include <type_traits>
+
+#include "kvq.cuh"
+
+namespace lumina {
+
+constexpr int KVQ_MAX_CTAS = 256;    // CTAs that may leave partial states
+constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of one sequence the decode kernel takes at most
+
+struct AttendArgs {
+  KvqView v;
+  const void* q;
+  void* out;
+  size_t ldq, ldo;
+  int nh, G;
+  float scale, cap;
+  const float* slopes;
+  const int* prefix;
+  int window;
+  int few;        // sequences of up to this many packed rows (rows x G) are the decode kernel's
+  int min_cells;  // decode: cells per CTA at least
+  float* ws;      // partial states
+  int* tickets;   // one per CTA, zero between launches
+  long long spin;
+};
+
+// sequences of up to a.few packed rows, at most max_packed of them (kvq_decode.cu)
+template <int HD, int BITS, typename T>
+int kvq_decode_launch(AttendArgs a, int max_packed, cudaStream_t s);
+
+// workspace: tickets, then partial states
+constexpr size_t KVQ_WS_TICKETS = 4096;
+inline size_t kvq_ws_bytes() {
+  return KVQ_WS_TICKETS + (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2) * 4;
+}
+
+// rows of sequence s as the batch says (0 where row_start is out of order)
+__device__ __forceinline__ int kvq_seq_rows(const KvqView& v, int s, int& first, bool report = true) {
+  first = __ldg(v.row_start + s);
+  const int end = __ldg(v.row_start + s + 1);
+  if (first < 0 || end < first || end > v.n_rows || end - first > v.max_rows) {
+    if (report) kvq_fault(v, KVQ_FAULT_DATA);
+    return 0;
+  }
+  return end - first;
+}
+
+__device__ __forceinline__ void kvq_store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void kvq_store4(__half* p, float a, float b, float c, float d) {
+  const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
+template <int N, int I = 0, typename Fn>
+__device__ __forceinline__ void static_for(Fn&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    static_for<N, I + 1>(f);
+  }
+}
+
+}  // namespace lumina

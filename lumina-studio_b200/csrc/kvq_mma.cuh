@@ -31,6 +31,16 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// tanh by 1 - 2 / (1 + e^2x): absolute error near 2^-23
+__device__ __forceinline__ float tanh_fast(float x) {
+  return fmaf(-2.f, rcp_approx(1.f + ex2(2.f * KVQ_LOG2E * x)), 1.f);
+}
+// 8 x 8 fp16 tile: (row g, columns 2t, 2t + 1) per lane -> (column g, rows 2t, 2t + 1)
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -90,13 +100,24 @@ struct KvqFrag {
       w[0] = q.x; w[1] = q.y;
     }
   }
-  // B fragment of step kk
-  template <int kk>
+  // fragment of step kk: k-indices e = 0, 1 in b0 and 2, 3 in b1. OFFSET
+  // leaves the fp16 numbers that hold the codes as they are, for callers that
+  // take the offset out of the product: 1152 + c (int8); 1024 + c in b0 and
+  // 1024 + 16 c in b1 (int4). Otherwise c (int8) or 2 c - 15 (int4).
+  template <int kk, bool OFFSET = false>
   __device__ static __forceinline__ void k_frag(const uint32_t (&w)[KW], uint32_t& b0, uint32_t& b1) {
-    if constexpr (BITS == 8) {
+    if constexpr (BITS == 8 && OFFSET) {
+      const uint32_t f = w[kk] ^ 0x80808080u;
+      b0 = __byte_perm(f, 0x64646464u, 0x4140);
+      b1 = __byte_perm(f, 0x64646464u, 0x4342);
+    } else if constexpr (BITS == 8) {
       const uint32_t f = w[kk] ^ 0x80808080u;
       b0 = s8_pair<0x4140>(f);
       b1 = s8_pair<0x4342>(f);
+    } else if constexpr (OFFSET) {
+      const uint32_t v = (kk & 1) ? w[kk >> 1] >> 8 : w[kk >> 1];
+      b0 = (v & 0x000F000Fu) | H_1024;
+      b1 = (v & 0x00F000F0u) | H_1024;
     } else {
       const uint32_t v = w[kk >> 1];
       b0 = u4_pair((kk & 1) ? v >> 4 : v << 4);

@@ -428,13 +428,17 @@ def test_out_of_range_data_is_reported(sv):
     kv = dev(rng.standard_normal((3, n_kv * hd)).astype(np.float32))
     cs = dev(np.ones((200, hd // 2), np.float32))
     good = pool.attend(batch_of(sv, [1, 1, 1], lens, table), q).clone()
+
+    def served(out, good):  # where the keys are split follows every length, so sums may round differently
+        return all(rel(out[i].cpu().numpy(), good[i].cpu().numpy()) < TOL["float32"] for i in (0, 2))
+
     assert cuda.fault_status(0) == 0
     bad_table = table.copy()
     bad_table[1] = [n_pages, -1, 1 << 30, n_pages + 5, 7, 7, 7][:table.shape[1]]
     bad = batch_of(sv, [1, 1, 1], lens, bad_table)
     out = pool.attend(bad, q)
     assert cuda.fault_status(0) == sv.FAULT_DATA
-    assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+    assert served(out, good)
     before = data.clone()
     pool.append(bad, q, kv, kv, cs, cs)
     assert cuda.fault_status(0) == sv.FAULT_DATA
@@ -447,7 +451,7 @@ def test_out_of_range_data_is_reported(sv):
     far = batch_of(sv, [1, 1, 1], [100, 10 ** 6, 70], table)
     out = pool.attend(far, q)
     assert cuda.fault_status(0) == sv.FAULT_DATA
-    assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+    assert served(out, good)
     pool.append(batch_of(sv, [1, 1, 1], lens, table), q, kv, kv, cs[:80].contiguous(), cs[:80].contiguous())
     assert cuda.fault_status(0) == sv.FAULT_DATA
 
