@@ -7,7 +7,7 @@
 
 namespace lumina {
 
-constexpr int KVQ_MAX_CTAS = 256;    // CTAs that may leave partial states
+constexpr int KVQ_MAX_CTAS = 320;    // CTAs that may leave partial states
 constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of one sequence the decode kernel takes at most
 
 struct AttendArgs {

@@ -9,8 +9,11 @@
 // in CTA order (the result does not depend on who that is).
 //
 // Every warp streams its own cells (every W-th of the CTA's segment) through
-// its own ring of shared-memory slots with bulk copies, across task
-// boundaries, and computes on its own: the scores transposed, S^T = K Q^T
+// its own ring of shared-memory slots, across task boundaries, and computes
+// on its own. The copies are cp.async of 16 bytes per lane: a cell is 2 to 4
+// KB, so a bulk copy per piece with its barrier cost one lane more
+// instructions than the whole warp now spends (608 -> see below), and each
+// chunk can land where the fragment loads meet no bank conflict. The math is the scores transposed, S^T = K Q^T
 // and O^T = V^T P^T with mma.sync m16n8k16, so that 16 keys (or dims) fill
 // the tensor pipe's 16 rows and the few query rows its 8 columns. Codes go
 // from shared memory to fragments in registers; the scales stay outside the
@@ -23,7 +26,6 @@
 #include <cfloat>
 #include <type_traits>
 
-#include "gemv_impl.cuh"
 #include "kvq_attend.cuh"
 #include "kvq_mma.cuh"
 
@@ -31,20 +33,30 @@ namespace lumina {
 
 namespace {
 
+// 16 bytes global -> shared, asynchronously
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 template <int HD, int BITS, int NR>
 struct DecCfg {
   using F = KvqFrag<HD, BITS>;
-  static constexpr int W = 16 / NR;             // warps: W x NR octets of rows fill the merge slabs
+  static constexpr int W = 8 / NR;              // warps: W x NR octets of rows fill the merge slabs
+  static constexpr int PER_SM = 2;              // CTAs per SM: one computes while the other merges
   static constexpr int THREADS = 32 * W;
   static constexpr int R = 8 * NR;              // packed rows
   static constexpr int SLOT = 16 * (2 * F::NB + 8);  // 16 keys: K codes, V codes, K scales, V scales
   static constexpr int LD = HD + 4;
   static constexpr int SLAB = R * LD * 4;       // one warp's O
-  static constexpr int RING = 227 * 1024 - W * SLAB - 20 * 1024;
+  // merging parts: 4-dim items of a row, Q threads per item, weights and joins
+  static constexpr int ITEMS = R * (HD / 4), Q = THREADS / ITEMS > 0 ? THREADS / ITEMS : 1;
+  static constexpr int JOIN = (R * KVQ_MAX_CTAS + (Q - 1) * ITEMS * 4) * 4;
+  static constexpr int MERGE = W * SLAB > JOIN ? W * SLAB : JOIN;
+  static constexpr int RING = 227 * 1024 / PER_SM - MERGE - 10 * 1024;
   static constexpr int S0 = RING / (W * SLOT);
   static constexpr int S = S0 > 6 ? 6 : S0;     // slots per warp
   static_assert(S >= 2, "at least one copy in flight beside the slot in use");
-  static constexpr size_t SMEM = (size_t)W * SLAB + (size_t)W * S * SLOT;  // + n_seq ints
+  static constexpr size_t SMEM = (size_t)MERGE + (size_t)W * S * SLOT;  // + n_seq ints
 };
 
 // One segment: cells [lo, hi) of the cell line of (KV head, sequence).
@@ -54,7 +66,7 @@ struct Seg {
 };
 
 template <int HD, int BITS, int NR, typename T>
-__global__ void __launch_bounds__(DecCfg<HD, BITS, NR>::THREADS, 1)
+__global__ void __launch_bounds__(DecCfg<HD, BITS, NR>::THREADS, (DecCfg<HD, BITS, NR>::PER_SM))
 kvq_decode_kernel(AttendArgs a) {
   using C = DecCfg<HD, BITS, NR>;
   using F = typename C::F;
@@ -65,21 +77,13 @@ kvq_decode_kernel(AttendArgs a) {
   constexpr bool OFFSET = !F32;
   extern __shared__ __align__(16) uint8_t sm[];
   float* slab = reinterpret_cast<float*>(sm);
-  uint8_t* ring_all = sm + W * C::SLAB;
-  int* line = reinterpret_cast<int*>(ring_all + W * S * C::SLOT);  // inclusive prefix of cells over sequences
-  __shared__ __align__(8) uint64_t bars[W][S];
+  uint8_t* ring_all = sm + C::MERGE;
+  int* cells = reinterpret_cast<int*>(ring_all + W * S * C::SLOT);  // inclusive prefix of cells over sequences
   __shared__ float m_s[W][R], l_s[W][R], M_s[R], L_s[R];
-  __shared__ int scan_s[W], last_s, dead_s;
+  __shared__ int scan_s[W], last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const KvqView& v = a.v;
   const int cap_tokens = v.pages_ld << v.page_shift;
-
-  if (lane == 0)
-    for (int i = 0; i < S; ++i) mbar_init(&bars[warp][i], 1);
-  if (tid == 0) {
-    dead_s = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
 
   // what the batch says about sequence s (0 rows: not this kernel's)
   auto describe = [&](int s, Seg& x, bool report) {
@@ -119,7 +123,7 @@ kvq_decode_kernel(AttendArgs a) {
       if (w < warp) before += scan_s[w];
       T_all += scan_s[w];
     }
-    if (s < v.n_seq) line[s] = (int)(before + inc);
+    if (s < v.n_seq) cells[s] = (int)(before + inc);
     __syncthreads();
   }
   if (T_all == 0 || T_all > 0x7fffffffLL) {
@@ -135,15 +139,15 @@ kvq_decode_kernel(AttendArgs a) {
   // the segment that starts at unit u of this CTA's range
   auto segment = [&](long long u, Seg& x) {
     const int kvh = (int)(u / Tn), c = (int)(u - (long long)kvh * Tn);
-    int lo = 0, hi = v.n_seq - 1;  // first s with line[s] > c
+    int lo = 0, hi = v.n_seq - 1;  // first s with cells[s] > c
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (line[mid] > c) hi = mid;
+      if (cells[mid] > c) hi = mid;
       else lo = mid + 1;
     }
     describe(lo, x, false);
     x.kvh = kvh;
-    const int base = lo ? line[lo - 1] : 0;
+    const int base = lo ? cells[lo - 1] : 0;
     x.lo = c - base;
     x.hi = (int)min((long long)x.total, x.lo + (u1 - u));
   };
@@ -171,44 +175,42 @@ kvq_decode_kernel(AttendArgs a) {
   };
   settle();
   int issued = 0;
-  // a cell without a readable page completes its slot without bytes; the
-  // consumer learns from `empty` (bit per slot)
+  // bit per slot: a cell without a readable page, nothing was copied
   unsigned empty = 0;
+  const int line = lane >> 3, lane_dst = line * 128 + (((lane & 7) ^ F::swz(line)) << 4);
   auto issue = [&]() {
-    const int slot = issued % S;
-    uint64_t* bar = &bars[warp][slot];
-    const bool good = (unsigned)pg < (unsigned)v.n_pages;
-    if (lane == 0) {
+    if (more) {
+      const int slot = issued % S;
+      const bool good = (unsigned)pg < (unsigned)v.n_pages;
       if (good) {
         const int j0 = (pc < ps.tp ? pc : pc - ps.tp + ps.tl) * 16, off = j0 & (P - 1);
-        const uint8_t* blk = v.pool + (size_t)pg * v.page_bytes + (size_t)ps.kvh * v.block_bytes;
-        uint8_t* dst = ring + slot * C::SLOT;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the warp's reads of the slot come first
-        mbar_expect_tx(bar, C::SLOT);
-        if (P == 16) {
-          bulk_g2s(dst, blk, C::SLOT, bar);
-        } else {
-          bulk_g2s(dst, blk + off * F::NB, 16 * F::NB, bar);
-          bulk_g2s(dst + 16 * F::NB, blk + (P + off) * F::NB, 16 * F::NB, bar);
-          bulk_g2s(dst + 32 * F::NB, blk + 2 * P * F::NB + 4 * off, 64, bar);
-          bulk_g2s(dst + 32 * F::NB + 64, blk + 2 * P * F::NB + 4 * (P + off), 64, bar);
+        const uint8_t* blk = v.pool + (size_t)pg * v.page_bytes + (uint32_t)ps.kvh * v.block_bytes;
+        const uint8_t* src = blk + off * F::NB + lane * 16;
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + slot * C::SLOT);
+        constexpr int CH = F::NB;  // chunks of 16 keys' codes
+#pragma unroll
+        for (int i = 0; i < CH / 32; ++i) {
+          // four lines further the swizzle flips bit 2 (128-byte rows) or repeats
+          const uint32_t d = dst + i * 512 + (F::NB == 128 && (i & 1) ? lane_dst ^ 64 : lane_dst);
+          cp_async16(d, src + i * 512);
+          cp_async16(d + 16 * F::NB, src + i * 512 + P * F::NB);
         }
-      } else {
-        if (pg != -2) kvq_fault(v, KVQ_FAULT_DATA);
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+        if (lane < 8)
+          cp_async16(dst + 32 * F::NB + lane * 16, blk + 2 * P * F::NB + 4 * off + (lane & 4 ? 4 * P : 0) + (lane & 3) * 16);
+      } else if (pg != -2 && lane == 0) {
+        kvq_fault(v, KVQ_FAULT_DATA);
       }
+      empty = (empty & ~(1u << slot)) | ((good ? 0u : 1u) << slot);
+      ++issued;
+      pc += W;
+      settle();
     }
-    empty = (empty & ~(1u << slot)) | ((good ? 0u : 1u) << slot);
-    ++issued;
-    pc += W;
-    settle();
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  __syncthreads();  // barriers initialized
-  while (more && issued < S) issue();
+  for (int i = 0; i < S - 1; ++i) issue();
 
   // ---- segments
-  int used = 0, dead_at = 0;
-  bool dead = false;
+  int used = 0;
   Seg x;
   for (long long u = u0; u < u1; u += x.hi - x.lo) {
     segment(u, x);
@@ -224,12 +226,13 @@ kvq_decode_kernel(AttendArgs a) {
       float q[KK][4];
       const T* src = static_cast<const T*>(a.q) + (size_t)(x.first + (ok ? i : 0)) * a.ldq +
                      (size_t)(x.kvh * a.G + (ok ? r - i * a.G : 0)) * HD;
+      F::load_q(src, t, q);
       float m = 0.f;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          q[kk][e] = ok ? (float)src[F::dim_of(t, kk, e)] : 0.f;
+          if (!ok) q[kk][e] = 0.f;
           m = fmaxf(m, fabsf(q[kk][e]));
         }
       // bring the row's largest value near 2^10: room for 16 q, and for what
@@ -289,30 +292,26 @@ kvq_decode_kernel(AttendArgs a) {
       for (int i = 0; i < NT / 2; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[r][i][c] = 0.f;
-    float m[NR][2], l[NR][2];
+    float m[NR][2], l[NR][2], ms[NR][2];  // ms: m, 0 while nothing was seen
 #pragma unroll
-    for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.f;
+    for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = ms[r][0] = ms[r][1] = 0.f;
     int ev = -100;         // V scales are taken relative to 2^ev
     float vmul = exp2i(7 + 100);
 
     for (int c = x.lo + warp; c < x.hi; c += W) {
       const int slot = used % S;
-      if (!dead && !mbar_wait_warp(&bars[warp][slot], (uint32_t)((used / S) & 1), a.spin, lane)) {
-        dead = true;
-        dead_at = used;
-        if (lane == 0) {
-          kvq_fault(v, KVQ_FAULT_WAIT);
-          dead_s = 1;
-        }
-      }
       ++used;
-      const bool skip = dead || ((empty >> slot) & 1u);
+      // one group per cell: all but the newest S - 2 have landed, for every lane
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();
+      issue();  // into the slot that the previous cell left
+      const bool skip = (empty >> slot) & 1u;
       const uint8_t* ks = ring + slot * C::SLOT;
       const int j0 = (c < x.tp ? c : c - x.tp + x.tl) * 16;
       if (!skip) {
         uint32_t kw[2][F::KW], vw[4][F::VW];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) F::load_k(ks + (h * 8 + g) * F::NB, t, kw[h]);
+        for (int h = 0; h < 2; ++h) F::load_k(ks, h * 8 + g, t, kw[h]);
         const float* sc = reinterpret_cast<const float*>(ks + 32 * F::NB);
         float sk[2] = {sc[g], sc[g + 8]}, sv[2] = {sc[16 + g], sc[24 + g]};
         const bool inner = j0 + 15 < x.len && ((j0 + 15 <= x.len - x.n && (a.window == 0 || j0 > x.len - 1 - a.window)) ||
@@ -343,7 +342,7 @@ kvq_decode_kernel(AttendArgs a) {
             }
           });
 #pragma unroll
-          for (int x4 = 0; x4 < 4; ++x4) F::load_v(ks + (16 + 2 * t + (x4 & 1) + 8 * (x4 >> 1)) * F::NB, g, vw[x4]);
+          for (int x4 = 0; x4 < 4; ++x4) F::load_v(ks + 16 * F::NB, 2 * t + (x4 & 1) + 8 * (x4 >> 1), g, vw[x4]);
 #pragma unroll
           for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -397,6 +396,7 @@ kvq_decode_kernel(AttendArgs a) {
               const float mn = fmaxf(m[r][c2], mx);
               fac[c2] = ex2(m[r][c2] - (mn == -INFINITY ? 0.f : mn));
               m[r][c2] = mn;
+              ms[r][c2] = mn == -INFINITY ? 0.f : mn;
               l[r][c2] *= fac[c2];
               fac[c2] *= es;
             }
@@ -411,8 +411,7 @@ kvq_decode_kernel(AttendArgs a) {
         for (int r = 0; r < NR; ++r) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float mm = m[r][e & 1];
-            const float y = ex2(p[r][e] - (mm == -INFINITY ? 0.f : mm));
+            const float y = ex2(p[r][e] - ms[r][e & 1]);
             l[r][e & 1] += y;
             // a masked key counts for nothing, whatever its scale holds
             p[r][e] = y == 0.f ? 0.f : y * (sv[e >> 1] * vmul);
@@ -442,8 +441,6 @@ kvq_decode_kernel(AttendArgs a) {
             }
           });
       }
-      __syncwarp();
-      if (more && !dead) issue();
     }
 
     // ---- merge the warps
@@ -499,7 +496,7 @@ kvq_decode_kernel(AttendArgs a) {
       }
       if (split) {
         *reinterpret_cast<float4*>(a.ws + my * part + (size_t)r * HD + d) = y;
-      } else if (!dead_s) {
+      } else {
         const float L = L_s[r], inv = L == 0.f ? 0.f : 1.0f / L;
         if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
         kvq_store4(static_cast<T*>(a.out) + (size_t)(x.first + r / a.G) * a.ldo + (size_t)(x.kvh * a.G + r % a.G) * HD + d,
@@ -539,7 +536,7 @@ kvq_decode_kernel(AttendArgs a) {
         }
         __syncthreads();
         // thread: 4 dims of a row, every Q-th part; the Q sums join in order
-        constexpr int ITEMS = R * (HD / 4), Q = C::THREADS / ITEMS > 0 ? C::THREADS / ITEMS : 1;
+        constexpr int ITEMS = C::ITEMS, Q = C::Q;
         float* join = slab + R * KVQ_MAX_CTAS;  // past the weights
         for (int i0 = 0; i0 < ITEMS * Q; i0 += C::THREADS) {
           const int i = (i0 + tid) % ITEMS, q = (i0 + tid) / ITEMS, r = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -562,7 +559,7 @@ kvq_decode_kernel(AttendArgs a) {
               y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
           }
-          if (r < rows && !dead_s) {
+          if (r < rows) {
             const float L = L_s[r], inv = L == 0.f ? 0.f : 1.0f / L;
             if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
             kvq_store4(static_cast<T*>(a.out) + (size_t)(x.first + r / a.G) * a.ldo +
@@ -575,9 +572,6 @@ kvq_decode_kernel(AttendArgs a) {
     }
     __syncthreads();  // slabs and statistics are free again
   }
-  // a warp that gave up lets its copies in flight land before it leaves
-  if (dead && lane == 0)
-    for (int i = dead_at; i < issued; ++i) mbar_wait_bounded(&bars[warp][i % S], (uint32_t)((i / S) & 1));
 }
 
 template <int HD, int BITS, int NR, typename T>
@@ -587,7 +581,7 @@ int decode_nr(const AttendArgs& a, cudaStream_t s) {
   const size_t smem = C::SMEM + (size_t)a.v.n_seq * 4;
   const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_decode");
   if (rc) return rc;
-  kern<<<min(sm_count(), KVQ_MAX_CTAS), C::THREADS, smem, s>>>(a);
+  kern<<<min(C::PER_SM * sm_count(), KVQ_MAX_CTAS), C::THREADS, smem, s>>>(a);
   LUMINA_LAUNCH_CHECK();
   return LUMINA_OK;
 }
