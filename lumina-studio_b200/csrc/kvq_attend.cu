@@ -19,22 +19,6 @@ namespace lumina {
 
 namespace {
 
-// the thread's code words of one key row as the pool stores it
-template <int HD, int BITS>
-__device__ __forceinline__ void row_k(const uint8_t* row, int t, uint32_t (&w)[KvqFrag<HD, BITS>::KW]) {
-#pragma unroll
-  for (int i = 0; i < KvqFrag<HD, BITS>::KW; ++i) {
-    constexpr int KW = KvqFrag<HD, BITS>::KW;
-    w[i] = reinterpret_cast<const uint32_t*>(row)[KW >= 4 ? ((i >> 2) * 4 + t) * 4 + (i & 3) : 2 * t + i];
-  }
-}
-template <int HD, int BITS>
-__device__ __forceinline__ void row_v(const uint8_t* row, int g, uint32_t (&w)[KvqFrag<HD, BITS>::VW]) {
-#pragma unroll
-  for (int i = 0; i < KvqFrag<HD, BITS>::VW; ++i)
-    w[i] = reinterpret_cast<const uint32_t*>(row)[g * KvqFrag<HD, BITS>::VW + i];
-}
-
 constexpr int AT_THREADS = 128;
 
 template <int HD, int BITS, typename T>
@@ -175,10 +159,10 @@ __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
     const int off = j0 & (P - 1);
     uint32_t kw[2][F::KW], vw[4][F::VW];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) row_k<HD, BITS>(blk + (size_t)(off + x * 8 + g) * F::NB, t, kw[x]);
+    for (int x = 0; x < 2; ++x) F::load_k(blk + (size_t)(off + x * 8 + g) * F::NB, t, kw[x]);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      row_v<HD, BITS>(blk + (size_t)(P + off + 2 * t + (x & 1) + 8 * (x >> 1)) * F::NB, g, vw[x]);
+      F::load_v(blk + (size_t)(P + off + 2 * t + (x & 1) + 8 * (x >> 1)) * F::NB, g, vw[x]);
     const float* sc = reinterpret_cast<const float*>(blk + 2 * P * F::NB) + off;
     float sk[4], sv[4];
 #pragma unroll
@@ -389,7 +373,7 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
   a.slopes = args->slopes_dev;
   a.prefix = args->prefix_dev;
   a.window = args->window;
-  a.min_cells = 16;
+  a.min_cells = 8;
   a.tickets = static_cast<int*>(args->workspace_dev);
   a.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(args->workspace_dev) + KVQ_WS_TICKETS);
   a.spin = wait_spin_limit();

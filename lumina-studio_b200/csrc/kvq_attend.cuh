@@ -7,7 +7,8 @@
 
 namespace lumina {
 
-constexpr int KVQ_MAX_CTAS = 320;    // CTAs that may leave partial states
+constexpr int KVQ_MAX_CTAS = 512;    // CTAs that may leave partial states (two each)
+constexpr int KVQ_FAN = 16;          // partial states that one CTA joins at a time
 constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of one sequence the decode kernel takes at most
 
 struct AttendArgs {
@@ -23,7 +24,7 @@ struct AttendArgs {
   int few;        // sequences of up to this many packed rows (rows x G) are the decode kernel's
   int min_cells;  // decode: cells per CTA at least
   float* ws;      // partial states
-  int* tickets;   // one per CTA, zero between launches
+  int* tickets;   // two per partial state, zero between launches
   long long spin;
 };
 
@@ -32,7 +33,7 @@ template <int HD, int BITS, typename T>
 int kvq_decode_launch(AttendArgs a, int max_packed, cudaStream_t s);
 
 // workspace: tickets, then partial states
-constexpr size_t KVQ_WS_TICKETS = 4096;
+constexpr size_t KVQ_WS_TICKETS = 4 * KVQ_MAX_CTAS * sizeof(int);
 inline size_t kvq_ws_bytes() {
   return KVQ_WS_TICKETS + (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2) * 4;
 }

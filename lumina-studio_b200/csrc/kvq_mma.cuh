@@ -117,28 +117,16 @@ struct KvqFrag {
           q[u * (RUN / 4) + kk][e] = x[BITS == 8 ? kk * 4 + e : (kk >> 1) * 8 + 2 * (kk & 1) + (e >> 1) + 4 * (e & 1)];
     }
   }
-  // Codes of 16 keys in shared memory: 128-byte lines of eight 16-byte
-  // chunks, chunk p of line L at p ^ swz(L), so that the lanes that load
-  // together (keys 2g.. for K, keys 2t.. for V) meet different banks.
-  __device__ static __forceinline__ int swz(int L) {
-    if constexpr (NB == 128) return (L & 6) ^ ((L & 1) << 2);
-    else return 2 * (L & 3);
-  }
-  // byte offset of 16-byte chunk c of key row r
-  __device__ static __forceinline__ int at(int r, int c) {
-    const int L = r * NB >> 7, p = (r & (128 / NB - 1)) * (NB / 16) + c;
-    return L * 128 + ((p ^ swz(L)) << 4);
-  }
-  // the thread's K code words of key row r (codes as laid out by `at`)
-  __device__ static __forceinline__ void load_k(const uint8_t* codes, int r, int t, uint32_t (&w)[KW]) {
+  // the thread's K code words of a key row in global memory
+  __device__ static __forceinline__ void load_k(const uint8_t* row, int t, uint32_t (&w)[KW]) {
     if constexpr (KW >= 4) {
 #pragma unroll
       for (int i = 0; i < KW / 4; ++i) {
-        const uint4 q = *reinterpret_cast<const uint4*>(codes + at(r, i * 4 + t));
+        const uint4 q = ldg_stream(row + (i * 4 + t) * 16);
         w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
       }
     } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(codes + at(r, t >> 1) + (t & 1) * 8);
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(row) + t);
       w[0] = q.x; w[1] = q.y;
     }
   }
@@ -166,15 +154,15 @@ struct KvqFrag {
       b1 = u4_pair((kk & 1) ? v >> 8 : v);
     }
   }
-  __device__ static __forceinline__ void load_v(const uint8_t* codes, int r, int g, uint32_t (&w)[VW]) {
+  __device__ static __forceinline__ void load_v(const uint8_t* row, int g, uint32_t (&w)[VW]) {
     if constexpr (VW == 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(codes + at(r, g));
+      const uint4 q = ldg_stream(row + g * 16);
       w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
     } else if constexpr (VW == 2) {
-      const uint2 q = *reinterpret_cast<const uint2*>(codes + at(r, g >> 1) + (g & 1) * 8);
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(row) + g);
       w[0] = q.x; w[1] = q.y;
     } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(codes + at(r, g >> 2) + (g & 3) * 4);
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(row) + g);
     }
   }
   // fp16 pairs (key a, key b) of dims DPW * j + i of the thread's run, where
