@@ -159,10 +159,10 @@ __global__ void __launch_bounds__(AT_THREADS) kvq_attend_kernel(AttendArgs a) {
     const int off = j0 & (P - 1);
     uint32_t kw[2][F::KW], vw[4][F::VW];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) F::load_k(blk + (size_t)(off + x * 8 + g) * F::NB, t, kw[x]);
+    for (int x = 0; x < 2; ++x) F::load_k(blk + (size_t)(off + x * 8 + g) * F::NB + F::k_lane(t), kw[x]);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      F::load_v(blk + (size_t)(P + off + 2 * t + (x & 1) + 8 * (x >> 1)) * F::NB, g, vw[x]);
+      F::load_v(blk + (size_t)(P + off + 2 * t + (x & 1) + 8 * (x >> 1)) * F::NB + F::v_lane(g), vw[x]);
     const float* sc = reinterpret_cast<const float*>(blk + 2 * P * F::NB) + off;
     float sk[4], sv[4];
 #pragma unroll

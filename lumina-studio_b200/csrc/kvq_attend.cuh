@@ -8,7 +8,7 @@
 namespace lumina {
 
 constexpr int KVQ_MAX_CTAS = 512;    // CTAs that may leave partial states (two each)
-constexpr int KVQ_FAN = 16;          // partial states that one CTA joins at a time
+constexpr int KVQ_FAN = 64;          // partial states that one CTA joins at a time
 constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of one sequence the decode kernel takes at most
 
 struct AttendArgs {

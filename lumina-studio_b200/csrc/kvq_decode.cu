@@ -39,7 +39,7 @@ struct DecCfg {
   static constexpr int CELL = 16 * NK;
   // registers decide: o and q of 8 NR rows and one cell's codes
   static constexpr int W = 4;                               // warps
-  static constexpr int PER_SM = NR == 1 && (BITS == 4 || HD == 64) && !F32 ? 3 : 2;  // CTAs per SM: some merge while others stream
+  static constexpr int PER_SM = 2;                          // CTAs per SM: one merges while the other streams
   static constexpr int THREADS = 32 * W;
   static constexpr int R = 8 * NR;                          // packed rows
   static constexpr int LD = HD + 4;
@@ -64,9 +64,15 @@ kvq_decode_kernel(AttendArgs a) {
   using C = DecCfg<HD, BITS, NR, F32>;
   using F = typename C::F;
   constexpr int KK = F::KK, NT = F::NT, W = C::W, R = C::R, NK = C::NK, CELL = C::CELL;
-  // fp16 rows: K codes enter with their fp16 offset (1024 + ...), which a
-  // start value of the accumulator takes off again; fp32 rows use exact codes
-  constexpr bool OFFSET = !F32;
+  // fp16 rows spend no instructions on making numbers of the codes:
+  //  int8 K  integer products with q as two int8 planes, q = a (256 h + l)
+  //  int4 K  codes with their fp16 offset (1024 + ...), which a start value of
+  //          the accumulator takes off again
+  //  V       raw codes as fp16 subnormals, zero point by one more product
+  // (q at 2^-16 of its largest value and sums of the offsets' size cost 2^-14
+  // of a score at most, below the fp16 rounding of p). fp32 rows use exact
+  // signed codes and split q and p.
+  constexpr bool FAST = !F32, IK = FAST && BITS == 8, OFFSET = FAST && BITS == 4;
   extern __shared__ __align__(16) uint8_t sm[];
   float* slab = reinterpret_cast<float*>(sm);
   int* cells = reinterpret_cast<int*>(sm + C::SMEM);  // inclusive prefix of cells over sequences
@@ -117,19 +123,18 @@ kvq_decode_kernel(AttendArgs a) {
     if (s < v.n_seq) cells[s] = (int)(before + inc);
     __syncthreads();
   }
-  if (T_all == 0 || T_all > 0x7fffffffLL) {
+  if (T_all == 0 || T_all * v.n_kv > 0x3fffffffLL) {
     if (T_all && tid == 0) kvq_fault(v, KVQ_FAULT_DATA);
     return;
   }
-  const int Tn = (int)T_all;
-  const long long U = (long long)Tn * v.n_kv;
-  const long long share = max((U + gridDim.x - 1) / gridDim.x, (long long)a.min_cells);
-  const long long u0 = blockIdx.x * share, u1 = min(U, u0 + share);
+  const unsigned Tn = (unsigned)T_all, U = Tn * (unsigned)v.n_kv;
+  const unsigned share = max((U + gridDim.x - 1) / gridDim.x, (unsigned)a.min_cells);
+  const unsigned u0 = blockIdx.x * share, u1 = min(U, u0 + share);
   if (u0 >= U) return;
 
   // the segment that starts at unit u of this CTA's range
-  auto segment = [&](long long u, Seg& x) {
-    const int kvh = (int)(u / Tn), c = (int)(u - (long long)kvh * Tn);
+  auto segment = [&](unsigned u, Seg& x) {
+    const int kvh = u / Tn, c = u - kvh * Tn;
     int lo = 0, hi = v.n_seq - 1;  // first s with cells[s] > c
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -140,19 +145,25 @@ kvq_decode_kernel(AttendArgs a) {
     x.kvh = kvh;
     const int base = lo ? cells[lo - 1] : 0;
     x.lo = c - base;
-    x.hi = (int)min((long long)x.total, x.lo + (u1 - u));
+    x.hi = min(x.total, x.lo + (int)(u1 - u));
   };
 
-  // ---- this warp's loads: `blk` is the tile to load next (the pool's first
-  // block where there is nothing to read), `have` says which tiles of the
-  // cell in registers hold keys; a cell's pages were asked for one cell earlier
+  // ---- this warp's loads: the cell to load next starts at key `jn`, its
+  // tile n holds keys if bit n of `have` is set (page 0 stands in where there
+  // is nothing to read); its pages were asked for one cell earlier. All
+  // addresses are this lane's own: kp (K codes) leads to the others.
   const int P = 1 << v.page_shift;
   const uint32_t page_bytes = (uint32_t)v.page_bytes;
+  const bool one_page = P >= CELL;
+  const int k_lane = g * F::NB + F::k_lane(t);
+  const int v_step = P * F::NB + 2 * t * F::NB + F::v_lane(g) - k_lane;  // kp -> its V codes
+  const int s_step = 2 * P * F::NB + 4 * g - k_lane;                     // page start's kp -> its first K scale
   Seg ps;
   segment(u0, ps);
-  long long pu = u0;
-  int pc = ps.lo + warp, pg[NK];
+  unsigned pu = u0;
+  int pc = ps.lo + warp, pg[NK], pj = 0;
   const int* table = v.pages + (size_t)ps.s * v.pages_ld;
+  const uint8_t* head = v.pool + (uint32_t)ps.kvh * v.block_bytes + k_lane;
   bool more = true;
   auto settle = [&]() {  // move to a cell of this warp and ask for its pages
     while (pc >= ps.hi) {
@@ -163,30 +174,44 @@ kvq_decode_kernel(AttendArgs a) {
       }
       segment(pu, ps);
       table = v.pages + (size_t)ps.s * v.pages_ld;
+      head = v.pool + (uint32_t)ps.kvh * v.block_bytes + k_lane;
       pc = ps.lo + warp;
     }
-    const int j0 = ps.at(pc) * CELL;
+    pj = ps.at(pc) * CELL;
+    pg[0] = pj < ps.len ? __ldg(table + ((unsigned)pj >> v.page_shift)) : -2;
+    if (!one_page) {
 #pragma unroll
-    for (int n = 0; n < NK; ++n) pg[n] = j0 + 16 * n < ps.len ? __ldg(table + ((j0 + 16 * n) >> v.page_shift)) : -2;
+      for (int n = 1; n < NK; ++n) pg[n] = pj + 16 * n < ps.len ? __ldg(table + ((unsigned)(pj + 16 * n) >> v.page_shift)) : -2;
+    }
   };
-  const uint8_t* blk[NK];  // K codes of the tile's first key
-  int soff[NK];            // from there to its K scale
+  const uint8_t *kp[NK], *sp[NK];
+  int jn = 0;
   unsigned have = 0;
+  auto place = [&](int n) {
+    const bool good = (unsigned)pg[n] < (unsigned)v.n_pages;
+    if (!good && more && pg[n] != -2 && lane == 0) kvq_fault(v, KVQ_FAULT_DATA);
+    const uint8_t* page = head + (uint64_t)(good ? (uint32_t)pg[n] : 0u) * page_bytes;
+    const uint32_t off = (pj + 16 * n) & (P - 1);
+    kp[n] = page + off * F::NB;
+    sp[n] = page + (int)(s_step + 4 * off);
+    have |= good ? 1u << n : 0u;
+  };
   auto advance = [&]() {
+    jn = pj;
     have = 0;
+    place(0);
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      const int off = (ps.at(pc) * CELL + 16 * n) & (P - 1);
-      const bool good = more && (unsigned)pg[n] < (unsigned)v.n_pages;
-      blk[n] = good ? v.pool + (size_t)((uint64_t)(uint32_t)pg[n] * page_bytes) + (uint32_t)ps.kvh * v.block_bytes + off * F::NB : v.pool;
-      soff[n] = good ? (2 * P - off) * F::NB + 4 * off : 2 * P * F::NB;
-      have |= good ? 1u << n : 0u;
-      if (more && !good && pg[n] != -2 && lane == 0) kvq_fault(v, KVQ_FAULT_DATA);
+    for (int n = 1; n < NK; ++n) {
+      if (one_page) {
+        kp[n] = kp[0] + 16 * n * F::NB;
+        sp[n] = sp[0] + 64 * n;
+        have |= have << n;
+      } else {
+        place(n);
+      }
     }
-    if (more) {
-      pc += W;
-      settle();
-    }
+    pc += W;
+    if (more) settle();
   };
   uint32_t kw[NK][2][F::KW], vw[NK][4][F::VW];
   float sk[NK][2], sv[NK][2];
@@ -194,22 +219,24 @@ kvq_decode_kernel(AttendArgs a) {
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) F::load_k(blk[n] + (h * 8 + g) * F::NB, t, kw[n][h]);
+      for (int h = 0; h < 2; ++h) F::load_k(kp[n] + h * 8 * F::NB, kw[n][h]);
   };
   auto load_v = [&]() {
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+    for (int n = 0; n < NK; ++n) {
+      const uint8_t* vp = kp[n] + v_step;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) F::load_v(blk[n] + (P + 2 * t + (i & 1) + 8 * (i >> 1)) * F::NB, g, vw[n][i]);
+      for (int i = 0; i < 4; ++i) F::load_v(vp + ((i & 1) + 8 * (i >> 1)) * F::NB, vw[n][i]);
+    }
   };
   auto load_s = [&]() {
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-      const float* sc = reinterpret_cast<const float*>(blk[n] + soff[n]) + g;
+      const float *sc = reinterpret_cast<const float*>(sp[n]), *sd = sc + P;
       sk[n][0] = __ldg(sc);
       sk[n][1] = __ldg(sc + 8);
-      sv[n][0] = __ldg(sc + P);
-      sv[n][1] = __ldg(sc + P + 8);
+      sv[n][0] = __ldg(sd);
+      sv[n][1] = __ldg(sd + 8);
     }
   };
   settle();
@@ -220,11 +247,11 @@ kvq_decode_kernel(AttendArgs a) {
 
   // ---- segments
   Seg x;
-  for (long long u = u0; u < u1; u += x.hi - x.lo) {
+  for (unsigned u = u0; u < u1; u += x.hi - x.lo) {
     segment(u, x);
     // this thread's rows: 8 o + g in the Q fragments, 8 o + 2 t + c in the scores
-    uint32_t qh[NR][KK][2], ql[F32 ? NR : 1][KK][2];
-    float qmul[NR][2], off[NR][2], slope[PLAIN ? 1 : NR][2];
+    uint32_t qh[NR][KK][2], ql[F32 ? NR : 1][KK][2];  // IK: [step][plane h: 0, 1 | plane l: 0, 1] in the 2 KK / 2 words
+    float qmul[NR][2], off[OFFSET ? NR : 1][2], slope[PLAIN ? 1 : NR][2];
     int pos[NR][2];
     const float scale = !PLAIN && a.cap > 0.f ? a.scale / a.cap : a.scale * KVQ_LOG2E;
 #pragma unroll
@@ -235,48 +262,63 @@ kvq_decode_kernel(AttendArgs a) {
       F::load_q(static_cast<const T*>(a.q) + (size_t)(x.first + (ok ? i : 0)) * a.ldq +
                     (size_t)(x.kvh * a.G + (ok ? r - i * a.G : 0)) * HD,
                 t, q);
-      float m = 0.f;
+      uint32_t top = 0;  // bits of the largest magnitude; past every finite one with an infinity or a NaN
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (!ok) q[kk][e] = 0.f;
-          m = fmaxf(m, fabsf(q[kk][e]));
+          top = max(top, __float_as_uint(q[kk][e]) & 0x7fffffffu);
         }
-      // bring the row's largest value near 2^10: room for 16 q, and for what
-      // hi leaves to lo
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const int ex = min(112, max(-112, (int)(__float_as_uint(m) >> 23) - 127));
-      const float up = exp2i(10 - ex);
-      float mul = scale * exp2i(ex - 10), sum = 0.f, lo_sum = 0.f;
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float mul, of = 0.f;
+      if constexpr (IK) {
+        const float am = __uint_as_float(top), to = top ? 32639.f / am : 0.f;
+        mul = top < 0x7f800000u ? scale * (am / 32639.f) : __uint_as_float(0x7fffffffu);
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
+        for (int kk = 0; kk < KK; ++kk) {
+          uint32_t h = 0, l = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q[kk][e] *= up;
-          sum += q[kk][e];
-          // int4: e = 0, 1 are low nibbles (1024 + c), 2 and 3 high ones (1024 + 16 c)
-          if (OFFSET && BITS == 4 && e < 2) {
-            lo_sum += q[kk][e];
-            q[kk][e] *= 16.f;
+          for (int e = 0; e < 4; ++e) {
+            const int i = __float2int_rn(q[kk][e] * to), hi = (i + 128) >> 8;
+            h |= (uint32_t)(hi & 0xFF) << (8 * e);
+            l |= (uint32_t)((i - 256 * hi) & 0xFF) << (8 * e);
+          }
+          // step kk / 2 takes word kk as its half kk % 2
+          qh[o][(kk >> 1) * 2][kk & 1] = h;
+          qh[o][(kk >> 1) * 2 + 1][kk & 1] = l;
+        }
+      } else {
+        // bring the row's largest value near 2^10: room for 16 q, and for
+        // what hi leaves to lo
+        const int ex = min(112, max(-112, (int)(top >> 23) - 127));
+        const float up = exp2i(10 - ex);
+        float sum = 0.f, lo_sum = 0.f;
+        mul = scale * exp2i(ex - 10);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            q[kk][e] *= up;
+            sum += q[kk][e];
+            // e = 0, 1 are low nibbles (1024 + c), 2 and 3 high ones (1024 + 16 c)
+            if (OFFSET && e < 2) {
+              lo_sum += q[kk][e];
+              q[kk][e] *= 16.f;
+            }
+          }
+          if constexpr (F32) {
+            qh[o][kk][0] = split_h2(q[kk][0], q[kk][1], ql[o][kk][0]);
+            qh[o][kk][1] = split_h2(q[kk][2], q[kk][3], ql[o][kk][1]);
+          } else {
+            qh[o][kk][0] = half2_bits(__floats2half2_rn(q[kk][0], q[kk][1]));
+            qh[o][kk][1] = half2_bits(__floats2half2_rn(q[kk][2], q[kk][3]));
           }
         }
-        if constexpr (F32) {
-          qh[o][kk][0] = split_h2(q[kk][0], q[kk][1], ql[o][kk][0]);
-          qh[o][kk][1] = split_h2(q[kk][2], q[kk][3], ql[o][kk][1]);
-        } else {
-          qh[o][kk][0] = half2_bits(__floats2half2_rn(q[kk][0], q[kk][1]));
-          qh[o][kk][1] = half2_bits(__floats2half2_rn(q[kk][2], q[kk][3]));
-        }
-      }
-      float of = 0.f;
-      if constexpr (OFFSET) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if constexpr (BITS == 8) {
-          of = -1152.f * sum;
-        } else {
+        if constexpr (OFFSET) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
           lo_sum += __shfl_xor_sync(0xffffffffu, lo_sum, 1);
           lo_sum += __shfl_xor_sync(0xffffffffu, lo_sum, 2);
           of = -(1024.f * (sum - lo_sum) + 16384.f * lo_sum + 120.f * sum);
@@ -287,7 +329,7 @@ kvq_decode_kernel(AttendArgs a) {
       for (int c = 0; c < 2; ++c) {
         const int rr = 8 * o + 2 * t + c;
         qmul[o][c] = __shfl_sync(0xffffffffu, mul, (2 * t + c) * 4);
-        off[o][c] = __shfl_sync(0xffffffffu, of, (2 * t + c) * 4);
+        if constexpr (OFFSET) off[o][c] = __shfl_sync(0xffffffffu, of, (2 * t + c) * 4);
         const int li = rr < x.n * a.G ? rr / a.G : 0;
         pos[o][c] = x.len - x.n + li;
         if constexpr (!PLAIN)
@@ -301,41 +343,76 @@ kvq_decode_kernel(AttendArgs a) {
       for (int i = 0; i < NT / 2; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[r][i][c] = 0.f;
+    float oz[FAST ? NR : 1][4];  // the zero points' product
+#pragma unroll
+    for (int r = 0; r < (FAST ? NR : 1); ++r) oz[r][0] = oz[r][1] = oz[r][2] = oz[r][3] = 0.f;
     float m[NR][2], l[NR][2], ms[NR][2];  // ms: m, 0 while nothing was seen
 #pragma unroll
     for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = ms[r][0] = ms[r][1] = 0.f;
     int ev = -100;  // V scales are taken relative to 2^ev
-    float vmul = exp2i(7 + 100);
+    const float sign = FAST && (g & 1) ? -1.f : 1.f;  // odd keys' p (v_raw)
+    float vmul = sign * exp2i(7 + 100);
 
-    const int see_all = x.len - x.n;                                          // keys up to here: every row
-    const int win_all = a.window ? x.len - a.window : 0;                        // keys from here: every row
+    // cells that start in [in_lo, in_hi] are seen by every row, as are those
+    // that end within the prefix
+    const int in_lo = a.window ? x.len - a.window : 0, in_hi = min(x.len - x.n + 1, x.len) - CELL, in_pre = x.pre - CELL;
     const int win_any = a.window ? x.len - x.n - a.window + 1 : -0x7fffffff;  // keys from here: some row
     for (int c = x.lo + warp; c < x.hi; c += W) {
-      const int j0 = x.at(c) * CELL;
+      const int j0 = jn;
       const unsigned held = have;
-      const bool inner = held == (1u << NK) - 1 && j0 + CELL <= x.len &&
-                         ((j0 + CELL - 1 <= see_all && j0 >= win_all) || j0 + CELL <= x.pre);
+      const bool inner = held == (1u << NK) - 1 && ((j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre);
       float p[NK][NR][4];  // [tile][row octet][key half * 2 + row c]
+      if constexpr (IK) {
+        // |sum h c| < 2^21: started at the bits of 1.5 * 2^23, the integer sum
+        // is the float 1.5 * 2^23 + sum
+        constexpr int MAGIC = 0x4B400000;
+        int dh[NK][NR][4], dl[NK][NR][4];
 #pragma unroll
-      for (int n = 0; n < NK; ++n)
+        for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+          for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[n][r][e] = OFFSET ? off[r][e & 1] : 0.f;
-      static_for<KK>([&](auto kc) {
-        constexpr int kk = decltype(kc)::value;
+            for (int e = 0; e < 4; ++e) dh[n][r][e] = dl[n][r][e] = MAGIC;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          uint32_t f[4];
-          F::template k_frag<kk, OFFSET>(kw[n][0], f[0], f[2]);
-          F::template k_frag<kk, OFFSET>(kw[n][1], f[1], f[3]);
+        for (int kk = 0; kk < KK / 2; ++kk)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            if constexpr (F32) mma_16816(p[n][r], f, ql[r][kk][0], ql[r][kk][1]);
-            mma_16816(p[n][r], f, qh[r][kk][0], qh[r][kk][1]);
+          for (int n = 0; n < NK; ++n) {
+            const uint32_t f[4] = {kw[n][0][2 * kk], kw[n][1][2 * kk], kw[n][0][2 * kk + 1], kw[n][1][2 * kk + 1]};
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              mma_16832_s8(dh[n][r], f, qh[r][2 * kk][0], qh[r][2 * kk][1]);
+              mma_16832_s8(dl[n][r], f, qh[r][2 * kk + 1][0], qh[r][2 * kk + 1][1]);
+            }
           }
-        }
-      });
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              p[n][r][e] = fmaf(__int_as_float(dh[n][r][e]) - 12582912.f, 256.f, __int_as_float(dl[n][r][e]) - 12582912.f);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[n][r][e] = OFFSET ? off[OFFSET ? r : 0][e & 1] : 0.f;
+        static_for<KK>([&](auto kc) {
+          constexpr int kk = decltype(kc)::value;
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            uint32_t f[4];
+            F::template k_frag<kk, OFFSET>(kw[n][0], f[0], f[2]);
+            F::template k_frag<kk, OFFSET>(kw[n][1], f[1], f[3]);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              if constexpr (F32) mma_16816(p[n][r], f, ql[r][kk][0], ql[r][kk][1]);
+              mma_16816(p[n][r], f, qh[r][kk][0], qh[r][kk][1]);
+            }
+          }
+        });
+      }
       advance();
       load_k();
       if (!inner) {  // scales of keys that no row sees do not count
@@ -388,7 +465,7 @@ kvq_decode_kernel(AttendArgs a) {
       float svm = 0.f;
 #pragma unroll
       for (int n = 0; n < NK; ++n) svm = fmaxf(svm, fmaxf(fabsf(sv[n][0]), fabsf(sv[n][1])));
-      bool up = svm * vmul > 128.f;
+      bool up = svm * fabsf(vmul) > 128.f;
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -404,7 +481,7 @@ kvq_decode_kernel(AttendArgs a) {
         const int en = max(ev, min(100, (int)(__float_as_uint(svm) >> 23) - 126));
         const float es = exp2i(max(-126, ev - en));
         ev = en;
-        vmul = exp2i(7 - en);
+        vmul = sign * exp2i(7 - en);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           float fac[2];
@@ -425,6 +502,10 @@ kvq_decode_kernel(AttendArgs a) {
           for (int i = 0; i < NT / 2; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[r][i][e] *= fac[e & 1];
+          if constexpr (FAST) {
+            oz[r][0] *= fac[0];
+            oz[r][1] *= fac[1];
+          }
         }
       }
       uint32_t pt[NK][NR][2], ptl[F32 ? NK : 1][F32 ? NR : 1][2];
@@ -464,16 +545,42 @@ kvq_decode_kernel(AttendArgs a) {
         for (int w = 0; w < F::VW; ++w)
           static_for<DPW / 2>([&](auto ic) {
             constexpr int i = 2 * decltype(ic)::value;
-            const uint32_t f[4] = {
-                F::template v_pair<i>(vw[n][0][w], vw[n][1][w]), F::template v_pair<i + 1>(vw[n][0][w], vw[n][1][w]),
-                F::template v_pair<i>(vw[n][2][w], vw[n][3][w]), F::template v_pair<i + 1>(vw[n][2][w], vw[n][3][w])};
+            if constexpr (FAST) {
+              const uint32_t f[4] = {
+                  F::template v_raw<i>(vw[n][0][w], vw[n][1][w]), F::template v_raw<i + 1>(vw[n][0][w], vw[n][1][w]),
+                  F::template v_raw<i>(vw[n][2][w], vw[n][3][w]), F::template v_raw<i + 1>(vw[n][2][w], vw[n][3][w])};
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              if constexpr (F32) mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
-              mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
+              for (int r = 0; r < NR; ++r) mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
+            } else {
+              const uint32_t f[4] = {
+                  F::template v_pair<i>(vw[n][0][w], vw[n][1][w]), F::template v_pair<i + 1>(vw[n][0][w], vw[n][1][w]),
+                  F::template v_pair<i>(vw[n][2][w], vw[n][3][w]), F::template v_pair<i + 1>(vw[n][2][w], vw[n][3][w])};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
+                mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
+              }
             }
           });
+      if constexpr (FAST) {
+        const uint32_t zp = half2_bits(__floats2half2_rn(F::RAW_ZERO[0], F::RAW_ZERO[1])), f[4] = {zp, zp, zp, zp};
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) mma_16816(oz[r], f, pt[n][r][0], pt[n][r][1]);
+      }
       load_v();
+    }
+    if constexpr (FAST) {  // sums of raw codes -> sums of values (int4: code = 2 c - 15, odd dims came times 16)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int i = 0; i < NT / 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float up = BITS == 8 ? 16777216.f : e < 2 ? 33554432.f : 2097152.f;
+            o[r][i][e] = fmaf(o[r][i][e], up, -(BITS == 8 ? 1.f : 2.f) * oz[r][e & 1]);
+          }
     }
 
     // ---- merge the warps
@@ -517,9 +624,9 @@ kvq_decode_kernel(AttendArgs a) {
     const int rows = x.n * a.G;
     // the task's first and last CTA, by the line alone; its parts' slots: a
     // CTA's piece that begins a task is the odd one of its two
-    const long long t0 = u - x.lo, cb = t0 / share, ce = (t0 + x.total - 1) / share;
+    const int cb = (u - x.lo) / share, ce = (u - x.lo + x.total - 1) / share;
     const size_t part = (size_t)R * (HD + 2);
-    auto slot_of = [&](long long p) { return 2 * (cb + p) + (p == 0 ? 1 : 0); };
+    auto slot_of = [&](int p) { return 2 * (cb + p) + (p == 0 ? 1 : 0); };
     auto finish = [&](int r, int d, float4 y) {  // dims d .. d + 3 of packed row r
       const float L = L_s[r], inv = 1.0f / L;
       if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);  // the row saw nothing
@@ -552,23 +659,38 @@ kvq_decode_kernel(AttendArgs a) {
         const int p0 = level == 0 ? (int)(blockIdx.x - cb) / KVQ_FAN * KVQ_FAN : 0, step = level == 0 ? 1 : KVQ_FAN;
         const int cnt = level == 0 ? min(KVQ_FAN, np - p0) : ng;
         const bool last_level = level == 1 || ng == 1;
-        __threadfence();
+        // the CTA's writes are ordered before the barrier, and by the fence
+        // of the thread that takes the ticket before the ticket
         __syncthreads();
         int* ticket = a.tickets + (level == 0 ? 0 : 2 * KVQ_MAX_CTAS) + slot_of(p0);
-        if (tid == 0) last_s = atomicAdd(ticket, 1) == cnt - 1;
+        if (tid == 0) {
+          __threadfence();
+          last_s = atomicAdd(ticket, 1) == cnt - 1;
+          if (last_s) {
+            __threadfence();
+            *ticket = 0;
+          }
+        }
         __syncthreads();
         if (!last_s) break;
-        __threadfence();
-        if (tid == 0) *ticket = 0;
         auto part_at = [&](int k) { return a.ws + slot_of(p0 + k * step) * part; };
         float* wt = slab;  // [row][cnt] weights of the parts (the slab's readers are past the barrier)
         for (int r = warp; r < rows; r += W) {
-          const float2 ml = lane < cnt ? __ldcg(reinterpret_cast<const float2*>(part_at(lane) + (size_t)R * HD) + r)
-                                       : make_float2(-INFINITY, 0.f);
-          const float M = warp_max(ml.x);
-          const float f = ex2(ml.x - (M == -INFINITY ? 0.f : M));
-          if (lane < cnt) wt[r * KVQ_FAN + lane] = f;
-          float L = lane < cnt ? f * ml.y : 0.f;
+          static_assert(KVQ_FAN == 64, "two parts per lane");
+          float2 ml[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = lane + 32 * h;
+            ml[h] = k < cnt ? __ldcg(reinterpret_cast<const float2*>(part_at(k) + (size_t)R * HD) + r) : make_float2(-INFINITY, 0.f);
+          }
+          const float M = warp_max(fmaxf(ml[0].x, ml[1].x)), Ms = M == -INFINITY ? 0.f : M;
+          float L = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = ex2(ml[h].x - Ms);
+            wt[r * KVQ_FAN + lane + 32 * h] = f;
+            if (lane + 32 * h < cnt) L += f * ml[h].y;
+          }
           L = warp_sum(L);
           if (lane == 0) {
             M_s[r] = M;
@@ -621,7 +743,6 @@ int decode_nr(const AttendArgs& a, cudaStream_t s) {
   const size_t smem = C::SMEM + (size_t)a.v.n_seq * 4;
   const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_decode");
   if (rc) return rc;
-  static_assert(KVQ_FAN <= 32, "one lane per part");
   kern<<<min(C::PER_SM * sm_count(), KVQ_MAX_CTAS), C::THREADS, smem, s>>>(a);
   LUMINA_LAUNCH_CHECK();
   return LUMINA_OK;

@@ -50,6 +50,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_16832_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 // (a, b) -> fp16 pair, and the fp16 pair of what it leaves
@@ -117,16 +123,18 @@ struct KvqFrag {
           q[u * (RUN / 4) + kk][e] = x[BITS == 8 ? kk * 4 + e : (kk >> 1) * 8 + 2 * (kk & 1) + (e >> 1) + 4 * (e & 1)];
     }
   }
-  // the thread's K code words of a key row in global memory
-  __device__ static __forceinline__ void load_k(const uint8_t* row, int t, uint32_t (&w)[KW]) {
+  // where a thread's code words of a key row start, and the words themselves
+  __device__ static __forceinline__ int k_lane(int t) { return t * (KW >= 4 ? 16 : 8); }
+  __device__ static __forceinline__ int v_lane(int g) { return g * VW * 4; }
+  __device__ static __forceinline__ void load_k(const uint8_t* p, uint32_t (&w)[KW]) {
     if constexpr (KW >= 4) {
 #pragma unroll
       for (int i = 0; i < KW / 4; ++i) {
-        const uint4 q = ldg_stream(row + (i * 4 + t) * 16);
+        const uint4 q = ldg_stream(p + i * 64);
         w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
       }
     } else {
-      const uint2 q = __ldg(reinterpret_cast<const uint2*>(row) + t);
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
       w[0] = q.x; w[1] = q.y;
     }
   }
@@ -154,28 +162,44 @@ struct KvqFrag {
       b1 = u4_pair((kk & 1) ? v >> 8 : v);
     }
   }
-  __device__ static __forceinline__ void load_v(const uint8_t* row, int g, uint32_t (&w)[VW]) {
+  __device__ static __forceinline__ void load_v(const uint8_t* p, uint32_t (&w)[VW]) {
     if constexpr (VW == 4) {
-      const uint4 q = ldg_stream(row + g * 16);
+      const uint4 q = ldg_stream(p);
       w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
     } else if constexpr (VW == 2) {
-      const uint2 q = __ldg(reinterpret_cast<const uint2*>(row) + g);
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
       w[0] = q.x; w[1] = q.y;
     } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(row) + g);
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
     }
   }
   // fp16 pairs (key a, key b) of dims DPW * j + i of the thread's run, where
-  // word j of each key holds DPW = 32 / BITS dims
+  // word j of each key holds DPW = 32 / BITS dims: c (int8), 2 c - 15 (int4)
   template <int i>
   __device__ static __forceinline__ uint32_t v_pair(uint32_t a, uint32_t b) {
     if constexpr (BITS == 8) {
-      // bytes (a_i, b_i) with 0x64 above each
       const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7362 : 0x5140);  // a_i' b_i' a_i'+1 b_i'+1
       return s8_pair<(i & 1) ? 0x4342 : 0x4140>(x ^ 0x80808080u);
     } else {
       const uint32_t x = __byte_perm(a, b, (i & 4) ? 0x7632 : 0x5410);
       return u4_pair((i & 3) == 0 ? x << 4 : x >> (4 * ((i & 3) - 1)));
+    }
+  }
+  // The same pairs as raw unsigned codes at the bottom of an fp16 mantissa,
+  // that is the subnormal code * 2^-24 (exact on the tensor pipe), the odd
+  // key's complemented: u = c + 128 and 255 - u (int8); c and 15 - c, for odd
+  // i times 16 (int4). With the odd keys' p negated, sum p (c - zero) =
+  // sum +-p u' - sum +-p w, w = RAW_ZERO of the key's parity, and the two
+  // sums stay small where sum p u would be 128 sum p.
+  static constexpr float RAW_ZERO[2] = {BITS == 8 ? 128.f : 7.5f, BITS == 8 ? 127.f : 7.5f};
+  template <int i>
+  __device__ static __forceinline__ uint32_t v_raw(uint32_t a, uint32_t b) {
+    if constexpr (BITS == 8) {
+      const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7632 : 0x5410);  // a_i' a_i'+1 | b_i' b_i'+1
+      return (((i & 1) ? x >> 8 : x) ^ 0x007F0080u) & 0x00FF00FFu;
+    } else {
+      const uint32_t x = __byte_perm(a, b, (i & 4) ? 0x7632 : 0x5410);
+      return (((i & 2) ? x >> 8 : x) ^ 0xFFFF0000u) & ((i & 1) ? 0x00F000F0u : 0x000F000Fu);
     }
   }
 };
