@@ -32,10 +32,20 @@ struct AttendArgs {
 template <int HD, int BITS, typename T>
 int kvq_decode_launch(AttendArgs a, int max_packed, cudaStream_t s);
 
+// sequences of more than a.few packed rows (kvq_chunk.cu)
+template <int HD, int BITS, typename T>
+int kvq_chunk_launch(AttendArgs a, cudaStream_t s);
+
+constexpr int KVQ_MAX_BLOCKS = 2048;  // row blocks whose key tiles the chunk kernel lines up
+constexpr int KVQ_CHUNK_CTAS = 160;   // CTAs of the chunk kernel at most
+constexpr int KVQ_CHUNK_ROWS = 256;   // packed rows of its partial states
+
 // workspace: tickets, then partial states
 constexpr size_t KVQ_WS_TICKETS = 4 * KVQ_MAX_CTAS * sizeof(int);
 inline size_t kvq_ws_bytes() {
-  return KVQ_WS_TICKETS + (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2) * 4;
+  const size_t decode = (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2) * 4;
+  const size_t chunk = (size_t)KVQ_CHUNK_CTAS * 2 * KVQ_CHUNK_ROWS * (128 + 2) * 4;
+  return KVQ_WS_TICKETS + (decode > chunk ? decode : chunk);
 }
 
 // rows of sequence s as the batch says (0 where row_start is out of order)

@@ -1,0 +1,822 @@
+// Attention of sequences with many new rows (prompt chunks, long drafts)
+// over quantized KV pages, on the 5th-gen tensor cores.
+//
+// A task is one (KV head, sequence, block of packed query rows); packed row r
+// is local row r / G, head r % G, so the G query heads that share a KV head
+// share its dequantized tiles. Key tiles of 128:
+//   S = Q K^T   tcgen05.mma, Q and K fp16 in shared memory, S in tensor memory
+//   P = 2^(x - ref) * (V scale), fp16, over S's own columns in tensor memory
+//   O += P V    tcgen05.mma, P from tensor memory, V fp16 in shared memory
+// K and V codes are small integers, exact in fp16; the scales stay outside:
+// a key's K scale multiplies its score column, its V scale its probability.
+// fp32 rows send Q and P as two fp16 parts (hi + lo, about 22 bits) through
+// the same tiles.
+//
+// One CTA per SM, 13 warps:
+//   warps 0-3, 4-7  softmax of row tile 0 and 1: a thread is a row, so
+//                   maximum and sum need no shuffles
+//   warps 8-11      codes from global memory to fp16 tiles (128-byte swizzle)
+//   warp 12         issues every MMA, owns the tensor memory
+// The two row tiles take turns on the tensor pipe: while one's S is being
+// exponentiated the other's products run. With at most 128 packed rows (and
+// always for fp32 rows) both softmax groups hold the SAME rows and take
+// alternate key tiles, and merge at the end.
+//
+// The reference exponent of a row (ref = maximum - 7 + exponent of the V
+// scales) moves only when a score passes the maximum by 2^8 or a V scale its
+// exponent; only then O is rescaled in tensor memory.
+//
+// The key tiles of all tasks form one line that the CTAs share evenly; tasks
+// that span CTAs leave partial states in the workspace, joined in part order
+// by the CTA that arrives last. With more row blocks than the line holds,
+// CTAs take whole tasks instead.
+//
+// Waits are bounded: one that gives up sets bit 5 of the device fault word,
+// every role leaves its loop, and the CTA frees its tensor memory and exits.
+#include <cfloat>
+#include <type_traits>
+
+#include "gemv_impl.cuh"
+#include "kvq_attend.cuh"
+#include "kvq_mma.cuh"
+
+namespace lumina {
+
+namespace {
+
+constexpr int CK_KEYS = 128;                // keys per tile
+constexpr int CK_DEQ = 8, CK_MMA = 12;      // first warp of the roles
+constexpr int CK_THREADS = 32 * (CK_MMA + 1);
+constexpr int CK_TILE = 128 * 128;          // bytes of a [128 rows][64 fp16] block
+constexpr uint32_t CK_S = 0, CK_O = 256;    // tensor memory columns: S tiles, O tiles, 128 apart
+
+template <int HD>
+struct CkCfg {
+  static constexpr int BLKS = HD / 64;               // 64-dim blocks of a tile
+  static constexpr int BYTES = BLKS * CK_TILE;       // one K, V or Q tile
+  static constexpr int Q_BYTES = 2 * 128 * HD * 2 > 128 * HD * 4 ? 2 * 128 * HD * 2 : 128 * HD * 4;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * BYTES, OFF_SC = OFF_V + 2 * BYTES;
+  static constexpr int OFF_LINE = OFF_SC + 2 * 2 * CK_KEYS * 4;  // [stage][K | V scale][key]
+  static constexpr size_t SMEM = OFF_LINE + (size_t)KVQ_MAX_BLOCKS * 4 + 1024;  // + n_seq ints
+};
+
+__device__ __forceinline__ void ck_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ck_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ck_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ck_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ck_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, int acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void ck_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, int acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// shared-memory descriptors, 128-byte swizzle. K-major: 8-row groups 1024
+// bytes apart. MN-major (V: the dims are contiguous): 64-dim blocks CK_TILE
+// bytes apart (leading offset), 8-key groups 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t ck_desc(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// fp16 A and B, fp32 D, M = 128; bit 16: B is MN-major
+__host__ __device__ constexpr uint32_t ck_idesc(int N, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void ck_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ck_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void ck_st32(uint32_t addr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+      "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+      "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void ck_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One segment: key tiles [lo, hi) of one task.
+struct CkSeg {
+  int kvh, s, first, n, len, pre;
+  int row0, rows;         // packed rows of the block
+  int tp, tl;             // tiles that the prefix shows; first tile that the window shows
+  int lo, hi, total;
+  bool alt;               // both softmax groups hold the same rows, alternate key tiles
+  __device__ __forceinline__ int key(int c) const { return (c < tp ? c : c - tp + tl) * CK_KEYS; }
+};
+
+template <int HD, int BITS, typename T>
+__global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) {
+  using C = CkCfg<HD>;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int BM = F32 ? 128 : 256;                    // packed rows of a block
+  constexpr int NB = HD * BITS / 8;                      // code bytes of a key
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* scale_s = reinterpret_cast<float*>(sm + C::OFF_SC);
+  int* line = reinterpret_cast<int*>(sm + C::OFF_LINE);  // inclusive prefix of tiles over blocks
+  int* blocks = line + KVQ_MAX_BLOCKS;                   // inclusive prefix of blocks over sequences
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, idle;
+  __shared__ uint32_t tmem_s, svm_s[2][4];
+  __shared__ int scan_s[CK_MMA + 1], abort_s, last_s;
+  __shared__ float m_s[128], l_s[128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const KvqView& v = a.v;
+  const int cap_tokens = v.pages_ld << v.page_shift;
+  volatile int* abort_v = &abort_s;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(&q_full, 8);
+    mbar_init(&idle, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_s = 0;
+  }
+  if (warp == CK_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+
+  // ---- the line of key tiles
+  auto block_scan = [&](int x, int& total) {  // inclusive over the CTA; two barriers
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) scan_s[warp] = inc;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w <= CK_MMA; ++w) {
+      if (w < warp) inc += scan_s[w];
+      total += scan_s[w];
+    }
+    __syncthreads();
+    return inc;
+  };
+  int NBt = 0;
+  for (int s0 = 0; s0 < v.n_seq; s0 += CK_THREADS) {
+    const int s = s0 + tid;
+    int first, nb = 0, total;
+    if (s < v.n_seq) {
+      const int n = kvq_seq_rows(v, s, first, blockIdx.x == 0);
+      if ((long long)n * a.G > a.few) nb = (int)(((long long)n * a.G + BM - 1) / BM);
+      const int len = __ldg(v.len + s);
+      if (nb && (len < 0 || len > cap_tokens) && blockIdx.x == 0) kvq_fault(v, KVQ_FAULT_DATA);
+    }
+    const int inc = block_scan(nb, total);
+    if (s < v.n_seq) blocks[s] = NBt + inc;
+    NBt += total;
+  }
+  __syncthreads();
+  // task b of the block line (any KV head): everything but kvh, lo, hi
+  auto describe = [&](int b, CkSeg& x) {
+    int lo = 0, hi = v.n_seq - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (blocks[mid] > b) hi = mid;
+      else lo = mid + 1;
+    }
+    x.s = lo;
+    x.n = kvq_seq_rows(v, lo, x.first, false);
+    x.len = min(cap_tokens, max(0, __ldg(v.len + lo)));
+    x.pre = a.prefix ? min(x.len, max(0, __ldg(a.prefix + lo))) : 0;
+    x.row0 = (b - (lo ? blocks[lo - 1] : 0)) * BM;
+    x.rows = min(BM, x.n * a.G - x.row0);
+    x.alt = x.rows <= 128;
+    const int p0 = x.len - x.n, p_lo = p0 + x.row0 / a.G, p_hi = p0 + (x.row0 + x.rows - 1) / a.G;
+    const int k_hi = min(x.len, max(0, p_hi + 1)), k_lo = a.window ? min(k_hi, max(0, p_lo - a.window + 1)) : 0;
+    x.tp = (x.pre + CK_KEYS - 1) / CK_KEYS;
+    x.tl = max(x.tp, k_lo / CK_KEYS);
+    x.total = max(1, x.tp + max(x.tl, (k_hi + CK_KEYS - 1) / CK_KEYS) - x.tl);
+  };
+  const bool whole = NBt > KVQ_MAX_BLOCKS;  // whole tasks: the line does not hold them
+  int Tn = NBt;                             // units of one KV head: tiles, or tasks
+  if (!whole) {
+    Tn = 0;
+    for (int b0 = 0; b0 < NBt; b0 += CK_THREADS) {
+      CkSeg x;
+      x.total = 0;
+      int total;
+      if (b0 + tid < NBt) describe(b0 + tid, x);
+      const int inc = block_scan(x.total, total);
+      if (b0 + tid < NBt) line[b0 + tid] = Tn + inc;
+      Tn += total;
+    }
+  }
+  ck_fence_before();
+  __syncthreads();
+  ck_fence_after();
+  const uint32_t tmem = tmem_s;
+  const long long U64 = (long long)Tn * v.n_kv;
+  const unsigned U = U64 > 0x3fffffffLL ? 0u : (unsigned)U64;
+  if (U64 > 0x3fffffffLL && tid == 0) kvq_fault(v, KVQ_FAULT_DATA);
+  const unsigned share = whole ? 1u : max((U + gridDim.x - 1) / gridDim.x, (unsigned)a.min_cells);
+  // units [u0, u1), or tasks u0, u0 + gridDim.x, ...
+  const unsigned u0 = whole ? blockIdx.x : min(U, blockIdx.x * share), u1 = whole ? U : min(U, u0 + share);
+  auto segment = [&](unsigned u, CkSeg& x) {  // returns the next segment's unit
+    x.kvh = u / Tn;
+    const int c = u - x.kvh * Tn;
+    if (whole) {
+      describe(c, x);
+      x.lo = 0;
+      x.hi = x.total;
+      return u + gridDim.x;
+    }
+    int lo = 0, hi = NBt - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (line[mid] > c) hi = mid;
+      else lo = mid + 1;
+    }
+    describe(lo, x);
+    x.lo = c - (lo ? line[lo - 1] : 0);
+    x.hi = (int)min((unsigned)x.total, x.lo + (u1 - u));
+    return u + (unsigned)(x.hi - x.lo);
+  };
+  auto give_up = [&]() {
+    if (!*abort_v) kvq_fault(v, KVQ_FAULT_WAIT);
+    *abort_v = 1;
+  };
+  // a whole warp waits; false when this wait or any role gave up
+  auto wait = [&](uint64_t* bar, unsigned phase) {
+    const bool in = mbar_wait_warp(bar, phase & 1, a.spin, lane);
+    if (!in && lane == 0) give_up();
+    return !__any_sync(0xffffffffu, !in || *abort_v);
+  };
+  const int P = 1 << v.page_shift;
+
+  if (warp >= CK_DEQ && warp < CK_MMA) {
+    // ======== codes -> fp16 tiles. A row is LPR 16-byte words of codes, one
+    // lane each; a pass of the 128 threads covers 128 / LPR rows.
+    constexpr int LPR = NB / 16, RPP = 128 / LPR, NP = LPR;
+    const int dt = tid - 32 * CK_DEQ, dw = warp - CK_DEQ;
+    const int wr = dt / LPR, wc = dt % LPR;
+    unsigned fill = 0;  // tiles filled so far (stage = fill & 1)
+    bool dead = false;
+    for (unsigned u = u0; u < u1 && !dead;) {
+      CkSeg x;
+      u = segment(u, x);
+      const uint8_t* base = v.pool + (size_t)x.kvh * v.block_bytes;
+      const int* table = v.pages + (size_t)x.s * v.pages_ld;
+      const int win_any = a.window ? x.len - x.n + x.row0 / a.G - a.window + 1 : -0x7fffffff;
+      // lane i & 7 knows the page of 16-key group i of a tile (-2: no key there)
+      auto ask = [&](int c) {
+        const int j = x.key(c) + (lane & 7) * 16;
+        return c < x.hi && j < x.len ? __ldg(table + (j >> v.page_shift)) : -2;
+      };
+      auto load = [&](int c, int pages, int isv, uint4 (&w)[NP]) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int r = p * RPP + wr;
+          const int pg = __shfl_sync(0xffffffffu, pages, r >> 4);
+          const int off = (x.key(c) + r) & (P - 1);
+          const bool good = (unsigned)pg < (unsigned)v.n_pages;
+          w[p] = ldg_stream(base + (size_t)(good ? pg : 0) * v.page_bytes + (size_t)((isv ? P : 0) + off) * NB + wc * 16);
+        }
+      };
+      auto store = [&](const uint4 (&w)[NP], uint8_t* tile) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int r = p * RPP + wr;
+          const uint32_t ws[4] = {w[p].x, w[p].y, w[p].z, w[p].w};
+          if constexpr (BITS == 8) {
+            // 16 dims: chunks 2 wc, 2 wc + 1 (of 8 dims) of block wc / 4
+            uint4 q[2];
+            uint32_t* qq = reinterpret_cast<uint32_t*>(q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t f = ws[i] ^ 0x80808080u;
+              qq[2 * i] = s8_pair<0x4140>(f);
+              qq[2 * i + 1] = s8_pair<0x4342>(f);
+            }
+            uint8_t* dst = tile + (wc >> 2) * CK_TILE + r * 128;
+            const int c0 = 2 * (wc & 3), sw = wc >> 2 & 1;  // the two blocks' stores take different banks
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<uint4*>(dst + (((c0 + (i ^ sw)) ^ (r & 7)) << 4)) = (i ^ sw) ? q[1] : q[0];
+          } else {
+            // 32 dims, one chunk per word, order 0 4 1 5 2 6 3 7 within it
+            uint8_t* dst = tile + (wc >> 1) * CK_TILE + r * 128;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t n = ws[i];
+              const uint4 q = make_uint4(u4_pair(n << 4), u4_pair(n), u4_pair(n >> 4), u4_pair(n >> 8));
+              *reinterpret_cast<uint4*>(dst + (((4 * (wc & 1) + i) ^ (r & 7)) << 4)) = q;
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      };
+      int pages = ask(x.lo);
+      uint4 cur[NP], nxt[NP];
+      load(x.lo, pages, 0, cur);
+      for (int c = x.lo; c < x.hi; ++c, ++fill) {
+        const int st = fill & 1;
+        const unsigned par = (fill >> 1) + 1;  // of the stage's previous release
+        // this key's scales (thread = key)
+        const int j = x.key(c) + dt;
+        const int pg = __shfl_sync(0xffffffffu, pages, (32 * dw + lane) >> 4);
+        const bool there = j < x.len && (unsigned)pg < (unsigned)v.n_pages;
+        if (j < x.len && !there && pg != -2) kvq_fault(v, KVQ_FAULT_DATA);
+        float sk = 0.f, sv = 0.f;
+        if (there && (j >= win_any || j < x.pre)) {
+          const float* sc = reinterpret_cast<const float*>(base + (size_t)pg * v.page_bytes + 2 * P * NB) + (j & (P - 1));
+          sk = __ldg(sc);
+          sv = __ldg(sc + P);
+        }
+        load(c, pages, 1, nxt);
+        const int next_pages = ask(c + 1);
+        if (fill >= 2 && !wait(&k_empty[st], par)) {
+          dead = true;
+          break;
+        }
+        store(cur, sm + C::OFF_K + st * C::BYTES);
+        __syncwarp();
+        if (lane == 0) ck_arrive(&k_full[st]);
+        if (c + 1 < x.hi) load(c + 1, next_pages, 0, cur);
+        if (fill >= 2 && !wait(&v_empty[st], par)) {
+          dead = true;
+          break;
+        }
+        scale_s[st * 256 + dt] = sk * (a.cap > 0.f ? a.scale / a.cap : a.scale * KVQ_LOG2E);
+        scale_s[st * 256 + 128 + dt] = sv;
+        // largest V scale of the tile (bits order like the values; a NaN does not count)
+        const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
+        const uint32_t mx = __reduce_max_sync(0xffffffffu, b > 0x7f800000u ? 0u : b);
+        if (lane == 0) svm_s[st][dw] = mx;
+        store(nxt, sm + C::OFF_V + st * C::BYTES);
+        __syncwarp();
+        if (lane == 0) ck_arrive(&v_full[st]);
+        pages = next_pages;
+      }
+    }
+  } else if (warp == CK_MMA) {
+    // ======== every MMA. Step j of a segment: softmax group j & 1, key tile
+    // j (alternating) or j / 2; S of step j + 2 follows P V of step j.
+    if (lane == 0) {
+      constexpr uint32_t ID_S = ck_idesc(128, false), ID_O = ck_idesc(HD, true);
+      const uint32_t sb = smem_u32(sm);
+      unsigned fill = 0, seg = 0, np[2] = {0, 0};
+      bool dead = false;
+      for (unsigned u = u0; u < u1 && !dead; ++seg) {
+        CkSeg x;
+        u = segment(u, x);
+        const int nt = x.hi - x.lo, J = x.alt ? nt : 2 * nt;
+        if (!mbar_wait_bounded(&q_full, seg & 1, a.spin) || *abort_v) {
+          give_up();
+          break;
+        }
+        ck_fence_after();
+        auto scores = [&](int j) {
+          const int t = j & 1, kt = x.alt ? j : j >> 1;
+          const unsigned f = fill + kt;
+          const int st = f & 1;
+          if (!mbar_wait_bounded(&k_full[st], (f >> 1) & 1, a.spin) || *abort_v) return false;
+          ck_fence_after();
+          const uint32_t ka = sb + C::OFF_K + st * C::BYTES;
+          const uint32_t qa = sb + (F32 || x.alt ? 0 : t * C::BYTES);
+          const uint32_t d = tmem + CK_S + t * 128;
+#pragma unroll
+          for (int part = 0; part < (F32 ? 2 : 1); ++part)  // fp32 rows: lo, then hi
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t o = (kk >> 2) * CK_TILE + (kk & 3) * 32;
+              ck_mma_ss(d, ck_desc(qa + (F32 ? (1 - part) * C::BYTES : 0) + o, 16), ck_desc(ka + o, 16), ID_S, (part | kk) != 0);
+            }
+          ck_commit(&s_full[t]);
+          if (x.alt || t == 1) ck_commit(&k_empty[st]);
+          return true;
+        };
+        for (int j = 0; j < 2 && j < J && !dead; ++j) dead = !scores(j);
+        for (int j = 0; j < J && !dead; ++j) {
+          const int t = j & 1, kt = x.alt ? j : j >> 1;
+          const unsigned f = fill + kt;
+          const int st = f & 1;
+          if (!mbar_wait_bounded(&v_full[st], (f >> 1) & 1, a.spin) || !mbar_wait_bounded(&p_full[t], np[t] & 1, a.spin) || *abort_v) {
+            dead = true;
+            break;
+          }
+          ++np[t];
+          ck_fence_after();
+          const uint32_t va = sb + C::OFF_V + st * C::BYTES;
+          const uint32_t d = tmem + CK_O + t * 128, p = tmem + CK_S + t * 128;
+          const int fresh = x.alt ? j < 2 : kt == 0;  // this group's first tile: O starts here
+#pragma unroll
+          for (int part = 0; part < (F32 ? 2 : 1); ++part)
+#pragma unroll
+            for (int kk = 0; kk < CK_KEYS / 16; ++kk)
+              ck_mma_ts(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + (F32 ? (1 - part) * 16 : 0), ck_desc(va + kk * 2048, CK_TILE), ID_O,
+                        !(fresh && part == 0 && kk == 0));
+          if (x.alt || t == 1) ck_commit(&v_empty[st]);
+          if (j + 2 >= J) ck_commit(&o_full[t]);
+          else dead = !scores(j + 2);
+        }
+        fill += nt;
+      }
+      if (dead) give_up();
+      ck_commit(&idle);  // completes once every MMA issued above is done
+    }
+  } else if (warp < CK_DEQ) {
+    // ======== softmax: thread = row
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // row of its tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_tm = tmem + lanes + CK_S + t * 128, o_tm = tmem + lanes + CK_O + t * 128;
+    unsigned fill = 0, ns = 0, no = 0;
+    bool dead = false;
+    auto pair_bar = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    for (unsigned u = u0; u < u1;) {
+      CkSeg x;
+      const unsigned un = segment(u, x);
+      const int nt = x.hi - x.lo;
+      const int pr = x.row0 + (x.alt ? 0 : t * 128) + row;  // packed row
+      const bool ok = pr < x.row0 + x.rows;
+      const int li = ok ? pr / a.G : x.row0 / a.G, head = x.kvh * a.G + (ok ? pr - li * a.G : 0);
+      const int pos = x.len - x.n + li;
+      // ---- Q to shared memory: this thread's row (alternating: group 1 writes half of it)
+      float rmul = 1.f;
+      {
+        const T* src = static_cast<const T*>(a.q) + (size_t)(x.first + li) * a.ldq + (size_t)head * HD;
+        uint8_t* dst = sm + (F32 || x.alt ? 0 : t * C::BYTES) + row * 128;
+        constexpr int CH = HD / 8;  // chunks of 8 dims
+        int c0 = 0, c1 = CH;
+        if constexpr (F32) {
+          uint32_t top = 0;
+#pragma unroll 4
+          for (int c = 0; c < HD / 4; ++c) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(src) + c);
+            top = max(max(top, __float_as_uint(f.x) & 0x7fffffffu), __float_as_uint(f.y) & 0x7fffffffu);
+            top = max(max(top, __float_as_uint(f.z) & 0x7fffffffu), __float_as_uint(f.w) & 0x7fffffffu);
+          }
+          const int ex = min(112, max(-112, (int)(top >> 23) - 127));
+          rmul = exp2i(ex - 13);
+        }
+        if (x.alt) {
+          c0 = t * (CH / 2);
+          c1 = c0 + CH / 2;
+        }
+        const float up = F32 ? __int_as_float((254 << 23) - __float_as_int(rmul)) : 1.f;  // 1 / rmul
+#pragma unroll 2
+        for (int c = c0; c < c1; ++c) {
+          float q[8];
+          if constexpr (F32) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(src) + 2 * c), g = __ldg(reinterpret_cast<const float4*>(src) + 2 * c + 1);
+            q[0] = f.x * up; q[1] = f.y * up; q[2] = f.z * up; q[3] = f.w * up;
+            q[4] = g.x * up; q[5] = g.y * up; q[6] = g.z * up; q[7] = g.w * up;
+          } else {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + c);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(bits_half2(ws[i]));
+              q[2 * i] = f.x;
+              q[2 * i + 1] = f.y;
+            }
+          }
+          if (!ok) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = 0.f;
+          }
+          constexpr int ord[8] = {0, BITS == 4 ? 4 : 1, BITS == 4 ? 1 : 2, BITS == 4 ? 5 : 3,
+                                  BITS == 4 ? 2 : 4, BITS == 4 ? 6 : 5, BITS == 4 ? 3 : 6, 7};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) hi[i] = split_h2(q[ord[2 * i]], q[ord[2 * i + 1]], lo[i]);
+          uint8_t* at = dst + (c >> 3) * CK_TILE + (((c & 7) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if constexpr (F32) *reinterpret_cast<uint4*>(at + C::BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ck_arrive(&q_full);
+      }
+      const float slope = a.slopes && ok ? __ldg(a.slopes + head) * KVQ_LOG2E : 0.f;
+      // keys that every row of the block sees; this row's own limits
+      const int p_lo = x.len - x.n + x.row0 / a.G, p_hi = x.len - x.n + (x.row0 + x.rows - 1) / a.G;
+      const int in_lo = a.window ? p_hi - a.window + 1 : 0, in_hi = min(p_lo + 1, x.len) - CK_KEYS, in_pre = x.pre - CK_KEYS;
+      const int r_lo = a.window ? pos - a.window + 1 : 0, r_hi = min(pos, x.len - 1);  // sees r_lo .. r_hi and 0 .. pre - 1
+      float m = -INFINITY, l = 0.f, ref = 0.f;
+      int ev = -100;
+      const int J = x.alt ? nt : 2 * nt;
+      for (int j = t; j < J && !dead; j += 2, ++ns) {
+        const int kt = x.alt ? j : j >> 1, j0 = x.key(x.lo + kt);
+        const unsigned f = fill + kt;
+        const int st = f & 1;
+        if (!wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns)) {
+          dead = true;
+          break;
+        }
+        ck_fence_after();
+        const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
+        const float4* vsc = ksc + 32;
+        const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
+        // x of columns 32 c .. 32 c + 31
+        auto scores = [&](int c, float (&z)[32]) {
+          ck_ld32(s_tm + 32 * c, z);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 k4 = ksc[8 * c + i];
+            if constexpr (F32) {
+              z[4 * i] *= k4.x * rmul; z[4 * i + 1] *= k4.y * rmul; z[4 * i + 2] *= k4.z * rmul; z[4 * i + 3] *= k4.w * rmul;
+            } else {
+              z[4 * i] *= k4.x; z[4 * i + 1] *= k4.y; z[4 * i + 2] *= k4.z; z[4 * i + 3] *= k4.w;
+            }
+          }
+          if (a.cap > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
+          }
+          if (a.slopes) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + 32 * c + i))), z[i]);
+          }
+          if (!inner) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int k = j0 + 32 * c + i;
+              if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
+            }
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float z[32];
+          scores(c, z);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, z[i]);
+        }
+        // a score past the maximum by 2^8, or a V scale past 2^ev
+        const uint32_t sb = max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3]));
+        const int en = max(ev, min(100, (int)(sb >> 23) - 126));
+        if (__any_sync(0xffffffffu, mx > m + 8.f || en > ev)) {
+          const float mn = fmaxf(m, mx);
+          const float rn = (mn == -INFINITY ? 0.f : mn) - 7.f + (float)en;
+          const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
+          m = mn;
+          ev = en;
+          ref = rn;
+          l *= fac;
+          if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              float o[32];
+              ck_ld32(o_tm + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= fac;
+              ck_st32(o_tm + 32 * c, o);
+            }
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float z[32];
+          scores(c, z);
+          uint32_t ph[16], pl[F32 ? 16 : 1];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 v4 = vsc[8 * c + i];
+            const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = ex2(z[4 * i + e] - ref);
+              l += y;
+              p[e] = y * vs[e];
+              if (!inner && y == 0.f) p[e] = 0.f;  // a masked key counts for nothing, whatever its scale holds
+            }
+            if constexpr (F32) {
+              ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
+              ph[2 * i + 1] = split_h2(p[2], p[3], pl[2 * i + 1]);
+            } else {
+              ph[2 * i] = half2_bits(__floats2half2_rn(p[0], p[1]));
+              ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
+            }
+          }
+          ck_st16(s_tm + 32 * c, ph);
+          if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
+        }
+        ck_wait_st();
+        ck_fence_before();
+        __syncwarp();
+        if (lane == 0) ck_arrive(&p_full[t]);
+      }
+      fill += nt;
+
+      // ---- the segment's end: O from tensor memory
+      const bool mine = J > t;  // this group had a tile
+      bool have = !dead;
+      if (mine && have) {
+        have = wait(&o_full[t], no);
+        ck_fence_after();
+      }
+      if (mine) ++no;
+      dead |= !have;
+      float* merge = reinterpret_cast<float*>(sm);  // the Q tiles are free: [128 rows][HD] floats, 16-byte chunks swizzled
+      auto at = [&](int r, int c4) { return reinterpret_cast<float4*>(merge + r * HD) + (c4 ^ (r & (HD / 4 - 1))); };
+      float f1 = 1.f;  // this group's weight (alternating: against the other's)
+      if (x.alt) {
+        // group 1 hands its state to group 0
+        if (t == 1) {
+          m_s[row] = mine ? m : -INFINITY;
+          l_s[row] = mine ? l : 0.f;
+          if (mine && have) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              float o[32];
+              ck_ld32(o_tm + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) *at(row, 8 * c + i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+          // the reference exponent stands in for the maximum: l and O are relative to it
+          m_s[row] = mine && m != -INFINITY ? ref : -INFINITY;
+        }
+        pair_bar();
+      }
+      const bool split = x.hi - x.lo < x.total;
+      const int cb = whole ? 0 : (u - x.lo) / share, ce = whole ? 0 : (u - x.lo + x.total - 1) / share;
+      auto slot_of = [&](int p) { return 2 * (cb + p) + (p == 0 ? 1 : 0); };
+      const size_t part = (size_t)BM * (HD + 2);
+      float* my_part = a.ws + slot_of(blockIdx.x - cb) * part;
+      // dims of output column 8 c + k (int4 codes unpack in another order)
+      auto put = [&](int packed, int c, const float (&o)[32], float inv) {  // columns 32 c .. + 31 of a packed row
+        const int i = packed / a.G;
+        T* dst = static_cast<T*>(a.out) + (size_t)(x.first + i) * a.ldo + (size_t)(x.kvh * a.G + packed - i * a.G) * HD + 32 * c;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int b = 8 * (k >> 1);
+          if constexpr (BITS == 4) {
+            // dim d of a group of 8 sits at column 2 (d & 3) + (d >> 2)
+            const int h = k & 1;
+            kvq_store4(dst + 4 * k, o[b + h] * inv, o[b + 2 + h] * inv, o[b + 4 + h] * inv, o[b + 6 + h] * inv);
+          } else {
+            kvq_store4(dst + 4 * k, o[4 * k] * inv, o[4 * k + 1] * inv, o[4 * k + 2] * inv, o[4 * k + 3] * inv);
+          }
+        }
+      };
+      if (!(x.alt && t == 1)) {
+        float R = m == -INFINITY ? -INFINITY : ref, f2 = 0.f, L = l;
+        if (x.alt) {
+          const float r1 = m_s[row], M = fmaxf(R, r1);
+          f1 = R == -INFINITY ? 0.f : ex2(R - M);
+          f2 = r1 == -INFINITY ? 0.f : ex2(r1 - M);
+          // a NaN sum stays one, whatever its weight
+          L = (l == l ? l * f1 : l) + (l_s[row] == l_s[row] ? l_s[row] * f2 : l_s[row]);
+          R = M;
+        }
+        const bool other = x.alt && J > 1;
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          float o[32];
+          ck_ld32(o_tm + 32 * c, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f1 == 0.f && L == L ? 0.f : o[i] * f1;
+          if (other) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 z = *at(row, 8 * c + i);
+              if (f2 != 0.f || L != L) {
+                o[4 * i] = fmaf(z.x, f2, o[4 * i]); o[4 * i + 1] = fmaf(z.y, f2, o[4 * i + 1]);
+                o[4 * i + 2] = fmaf(z.z, f2, o[4 * i + 2]); o[4 * i + 3] = fmaf(z.w, f2, o[4 * i + 3]);
+              }
+            }
+          }
+          if (L == 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (ok && !dead) {
+            if (split) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                __stcg(reinterpret_cast<float4*>(my_part + (size_t)(pr - x.row0) * HD + 32 * c) + i,
+                       make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+            } else {
+              put(pr, c, o, inv);
+            }
+          }
+        }
+        if (split && ok) __stcg(reinterpret_cast<float2*>(my_part + (size_t)BM * HD) + (pr - x.row0), make_float2(R, L));
+      }
+      ck_fence_before();
+      pair_bar();  // Q tiles, merge buffer and O are free for the next segment
+      if (split) {
+        if (tid == 0) {
+          __threadfence();
+          last_s = atomicAdd(a.tickets + slot_of(0), 1) == ce - cb;
+          if (last_s) {
+            __threadfence();
+            a.tickets[slot_of(0)] = 0;
+          }
+        }
+        pair_bar();
+        if (last_s) {
+          // thread: 4 dims of a row, the parts in order
+          const int np = ce - cb + 1;
+          for (int i = tid; i < x.rows * (HD / 4); i += 256) {
+            const int r = i / (HD / 4), d4 = i % (HD / 4);
+            float M = -INFINITY, L = 0.f;
+            for (int p = 0; p < np; ++p)
+              M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(a.ws + slot_of(p) * part + (size_t)BM * HD) + r).x);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int p = 0; p < np; ++p) {
+              const float* at_p = a.ws + slot_of(p) * part;
+              const float2 rl = __ldcg(reinterpret_cast<const float2*>(at_p + (size_t)BM * HD) + r);
+              const float4 z = __ldcg(reinterpret_cast<const float4*>(at_p + (size_t)r * HD) + d4);
+              const float w = rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M);
+              L += rl.y * w;
+              y.x = fmaf(z.x, w, y.x); y.y = fmaf(z.y, w, y.y); y.z = fmaf(z.z, w, y.z); y.w = fmaf(z.w, w, y.w);
+            }
+            const float inv = 1.0f / L;
+            if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+            else y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+            const int packed = x.row0 + r, li2 = packed / a.G;
+            T* dst = static_cast<T*>(a.out) + (size_t)(x.first + li2) * a.ldo + (size_t)(x.kvh * a.G + packed - li2 * a.G) * HD;
+            if constexpr (BITS == 4) {
+              // columns 4 d4 .. + 3 hold dims b + {0, 4, 1, 5} or b + {2, 6, 3, 7}
+              const int b = (d4 >> 1) * 8 + 2 * (d4 & 1);
+              dst[b] = (T)y.x; dst[b + 4] = (T)y.y; dst[b + 1] = (T)y.z; dst[b + 5] = (T)y.w;
+            } else {
+              kvq_store4(dst + 4 * d4, y.x, y.y, y.z, y.w);
+            }
+          }
+        }
+        pair_bar();
+      }
+      u = un;
+    }
+  }
+  ck_fence_before();
+  __syncthreads();
+  if (warp == CK_MMA) {
+    if (lane == 0) mbar_wait_bounded(&idle, 0u, MBAR_SPIN_LIMIT);  // no MMA may still write the memory that is freed
+    __syncwarp();
+    ck_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+}  // namespace
+
+template <int HD, int BITS, typename T>
+int kvq_chunk_launch(AttendArgs a, cudaStream_t s) {
+  using C = CkCfg<HD>;
+  auto kern = kvq_chunk_kernel<HD, BITS, T>;
+  a.min_cells = 2;
+  const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_chunk");
+  if (rc) return rc;
+  kern<<<min(sm_count(), KVQ_CHUNK_CTAS), CK_THREADS, C::SMEM + (size_t)a.v.n_seq * 4, s>>>(a);
+  LUMINA_LAUNCH_CHECK();
+  return LUMINA_OK;
+}
+template int kvq_chunk_launch<128, 8, __half>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<128, 8, float>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<128, 4, __half>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<128, 4, float>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<64, 8, __half>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<64, 8, float>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<64, 4, __half>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<64, 4, float>(AttendArgs, cudaStream_t);
+
+}  // namespace lumina
