@@ -12,18 +12,18 @@
 // fp32 rows send Q and P as two fp16 parts (hi + lo, about 22 bits) through
 // the same tiles.
 //
-// One CTA per SM, 13 warps:
+// One CTA per SM, 12 warps (168 registers a thread):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: a thread is a row, so
-//                   maximum and sum need no shuffles
+//                   maximum and sum need no shuffles; each group's first warp
+//                   issues the group's own MMAs, P V and then the next S
 //   warps 8-11      codes from global memory to fp16 tiles (128-byte swizzle)
-//   warp 12         issues every MMA, owns the tensor memory
 // The two row tiles take turns on the tensor pipe: while one's S is being
 // exponentiated the other's products run. With at most 128 packed rows (and
 // always for fp32 rows) both softmax groups hold the SAME rows and take
 // alternate key tiles, and merge at the end.
 //
-// The reference exponent of a row (ref = maximum - 7 + exponent of the V
-// scales) moves only when a score passes the maximum by 2^8 or a V scale its
+// The reference exponent of a row (its maximum and the exponent of the V
+// scales) moves only when P might leave fp16's range or a V scale passes its
 // exponent; only then O is rescaled in tensor memory.
 //
 // The key tiles of all tasks form one line that the CTAs share evenly; tasks
@@ -45,8 +45,15 @@ namespace lumina {
 namespace {
 
 constexpr int CK_KEYS = 128;                // keys per tile
-constexpr int CK_DEQ = 8, CK_MMA = 12;      // first warp of the roles
-constexpr int CK_THREADS = 32 * (CK_MMA + 1);
+constexpr int CK_DEQ = 8;                   // first warp that fills tiles
+constexpr int CK_THREADS = 384;
+// P is 2^LIFT at the maximum the reference was set by, and may grow to 2^15
+// (fp16's range) before the reference moves. fp32 rows need their small p's
+// low parts above fp16's subnormals, fp16 rows a rarely moving reference.
+template <bool F32>
+struct CkLift {
+  static constexpr float LIFT = F32 ? 10.f : 4.f, MARGIN = 15.f - LIFT;
+};
 constexpr int CK_TILE = 128 * 128;          // bytes of a [128 rows][64 fp16] block
 constexpr uint32_t CK_S = 0, CK_O = 256;    // tensor memory columns: S tiles, O tiles, 128 apart
 
@@ -101,9 +108,41 @@ __device__ __forceinline__ void ck_ld32(uint32_t addr, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// the loads issued so far are in their registers; v may be used after this
+__device__ __forceinline__ void ck_wait_ld(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void ck_get32(uint32_t addr, float (&v)[32]) {
+  ck_ld32(addr, v);
+  ck_wait_ld(v);
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 a, a, b, c;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ void ck_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -122,6 +161,12 @@ __device__ __forceinline__ void ck_st32(uint32_t addr, const float (&v)[32]) {
       "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
       : "memory");
 }
+// one lane of a converged warp, always the same
+__device__ __forceinline__ bool ck_elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void ck_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One segment: key tiles [lo, hi) of one task.
@@ -134,7 +179,7 @@ struct CkSeg {
   __device__ __forceinline__ int key(int c) const { return (c < tp ? c : c - tp + tl) * CK_KEYS; }
 };
 
-template <int HD, int BITS, typename T>
+template <int HD, int BITS, typename T, bool PLAIN>
 __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) {
   using C = CkCfg<HD>;
   constexpr bool F32 = sizeof(T) == 4;
@@ -145,9 +190,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
   float* scale_s = reinterpret_cast<float*>(sm + C::OFF_SC);
   int* line = reinterpret_cast<int*>(sm + C::OFF_LINE);  // inclusive prefix of tiles over blocks
   int* blocks = line + KVQ_MAX_BLOCKS;                   // inclusive prefix of blocks over sequences
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, idle;
-  __shared__ uint32_t tmem_s, svm_s[2][4];
-  __shared__ int scan_s[CK_MMA + 1], abort_s, last_s;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], o_full[2], turn[2], idle;
+  __shared__ uint32_t tmem_s, skm_s[2][4], svm_s[2][4];  // a tile's largest K and V scale, one per warp that filled it
+  __shared__ int scan_s[CK_THREADS / 32], abort_s, last_s;
   __shared__ float m_s[128], l_s[128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const KvqView& v = a.v;
@@ -158,18 +203,17 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&v_full[i], 4);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&k_empty[i], 2);  // two commits: one per group, or two of the one that used the stage
+      mbar_init(&v_empty[i], 2);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&turn[i], 1);
     }
-    mbar_init(&q_full, 8);
-    mbar_init(&idle, 1);
+    mbar_init(&idle, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_s = 0;
   }
-  if (warp == CK_MMA) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -185,7 +229,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
     if (lane == 31) scan_s[warp] = inc;
     __syncthreads();
     total = 0;
-    for (int w = 0; w <= CK_MMA; ++w) {
+    for (int w = 0; w < CK_THREADS / 32; ++w) {
       if (w < warp) inc += scan_s[w];
       total += scan_s[w];
     }
@@ -276,20 +320,31 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
     if (!*abort_v) kvq_fault(v, KVQ_FAULT_WAIT);
     *abort_v = 1;
   };
-  // a whole warp waits; false when this wait or any role gave up
+  // a whole warp waits; false when this wait or, meanwhile, any role gave up
   auto wait = [&](uint64_t* bar, unsigned phase) {
-    const bool in = mbar_wait_warp(bar, phase & 1, a.spin, lane);
+    bool in = false;
+    for (long long i = 0; i < a.spin; ++i) {
+      if (mbar_try_wait(bar, phase & 1)) {
+        in = true;
+        break;
+      }
+      if ((i & 1023) == 1023 && *abort_v) break;
+    }
+    in = __all_sync(0xffffffffu, in);
     if (!in && lane == 0) give_up();
-    return !__any_sync(0xffffffffu, !in || *abort_v);
+    return in;
   };
   const int P = 1 << v.page_shift;
 
-  if (warp >= CK_DEQ && warp < CK_MMA) {
+  if (warp >= CK_DEQ) {
     // ======== codes -> fp16 tiles. A row is LPR 16-byte words of codes, one
     // lane each; a pass of the 128 threads covers 128 / LPR rows.
     constexpr int LPR = NB / 16, RPP = 128 / LPR, NP = LPR;
     const int dt = tid - 32 * CK_DEQ, dw = warp - CK_DEQ;
-    const int wr = dt / LPR, wc = dt % LPR;
+    // 128-byte rows: eight consecutive lanes take half a row each of two
+    // neighbouring rows, whose stores meet different banks
+    const int wr = LPR == 8 ? dw * 4 + ((lane >> 2) & 1) + 2 * (lane >> 4) : dt / LPR;
+    const int wc = LPR == 8 ? (lane & 3) + 4 * ((lane >> 3) & 1) : dt % LPR;
     unsigned fill = 0;  // tiles filled so far (stage = fill & 1)
     bool dead = false;
     for (unsigned u = u0; u < u1 && !dead;) {
@@ -297,13 +352,14 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
       u = segment(u, x);
       const uint8_t* base = v.pool + (size_t)x.kvh * v.block_bytes;
       const int* table = v.pages + (size_t)x.s * v.pages_ld;
+      const float kmul = a.cap > 0.f ? a.scale / a.cap : a.scale * KVQ_LOG2E;
       const int win_any = a.window ? x.len - x.n + x.row0 / a.G - a.window + 1 : -0x7fffffff;
       // lane i & 7 knows the page of 16-key group i of a tile (-2: no key there)
       auto ask = [&](int c) {
         const int j = x.key(c) + (lane & 7) * 16;
         return c < x.hi && j < x.len ? __ldg(table + (j >> v.page_shift)) : -2;
       };
-      auto load = [&](int c, int pages, int isv, uint4 (&w)[NP]) {
+      auto load = [&](int c, int pages, bool isv, uint4 (&w)[NP]) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           const int r = p * RPP + wr;
@@ -329,10 +385,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
               qq[2 * i + 1] = s8_pair<0x4342>(f);
             }
             uint8_t* dst = tile + (wc >> 2) * CK_TILE + r * 128;
-            const int c0 = 2 * (wc & 3), sw = wc >> 2 & 1;  // the two blocks' stores take different banks
+            const int c0 = 2 * (wc & 3);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              *reinterpret_cast<uint4*>(dst + (((c0 + (i ^ sw)) ^ (r & 7)) << 4)) = (i ^ sw) ? q[1] : q[0];
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(dst + (((c0 + i) ^ (r & 7)) << 4)) = q[i];
           } else {
             // 32 dims, one chunk per word, order 0 4 1 5 2 6 3 7 within it
             uint8_t* dst = tile + (wc >> 1) * CK_TILE + r * 128;
@@ -346,123 +401,90 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       };
-      int pages = ask(x.lo);
-      uint4 cur[NP], nxt[NP];
-      load(x.lo, pages, 0, cur);
-      for (int c = x.lo; c < x.hi; ++c, ++fill) {
-        const int st = fill & 1;
-        const unsigned par = (fill >> 1) + 1;  // of the stage's previous release
-        // this key's scales (thread = key)
+      // order: K 0, K 1, V 0, K 2, V 1, ...: S of a tile is wanted before P V
+      // of the one before it. Codes and scales are in registers a tile ahead
+      // of their store, page numbers a tile ahead of that.
+      const int p0 = ask(x.lo);
+      int p1 = ask(x.lo + 1), p2 = ask(x.lo + 2);  // pages of tiles c + 1, c + 2
+      uint4 kw[NP], vw[NP];
+      float sk, sv;
+      auto load_s = [&](int c, int pages) {  // tile c's scales (thread = key)
         const int j = x.key(c) + dt;
-        const int pg = __shfl_sync(0xffffffffu, pages, (32 * dw + lane) >> 4);
+        const int pg = __shfl_sync(0xffffffffu, pages, dt >> 4);
         const bool there = j < x.len && (unsigned)pg < (unsigned)v.n_pages;
         if (j < x.len && !there && pg != -2) kvq_fault(v, KVQ_FAULT_DATA);
-        float sk = 0.f, sv = 0.f;
+        sk = sv = 0.f;
         if (there && (j >= win_any || j < x.pre)) {
           const float* sc = reinterpret_cast<const float*>(base + (size_t)pg * v.page_bytes + 2 * P * NB) + (j & (P - 1));
           sk = __ldg(sc);
           sv = __ldg(sc + P);
         }
-        load(c, pages, 1, nxt);
-        const int next_pages = ask(c + 1);
-        if (fill >= 2 && !wait(&k_empty[st], par)) {
-          dead = true;
-          break;
-        }
-        store(cur, sm + C::OFF_K + st * C::BYTES);
+      };
+      load(x.lo, p0, false, kw);
+      load(x.lo, p0, true, vw);
+      load_s(x.lo, p0);
+      auto fill_k = [&](int c, int next_pages) {
+        const unsigned f = fill + (c - x.lo);
+        if (f >= 2 && !wait(&k_empty[f & 1], (f >> 1) + 1)) return false;
+        store(kw, sm + C::OFF_K + (f & 1) * C::BYTES);
         __syncwarp();
-        if (lane == 0) ck_arrive(&k_full[st]);
-        if (c + 1 < x.hi) load(c + 1, next_pages, 0, cur);
-        if (fill >= 2 && !wait(&v_empty[st], par)) {
+        if (lane == 0) ck_arrive(&k_full[f & 1]);
+        if (c + 1 < x.hi) load(c + 1, next_pages, false, kw);
+        return true;
+      };
+      dead = !fill_k(x.lo, p1);
+      for (int c = x.lo; c < x.hi && !dead; ++c) {
+        const int p3 = ask(c + 3);
+        if (c + 1 < x.hi && !fill_k(c + 1, p2)) {
           dead = true;
           break;
         }
-        scale_s[st * 256 + dt] = sk * (a.cap > 0.f ? a.scale / a.cap : a.scale * KVQ_LOG2E);
+        const unsigned f = fill + (c - x.lo);
+        const int st = f & 1;
+        if (f >= 2 && !wait(&v_empty[st], (f >> 1) + 1)) {
+          dead = true;
+          break;
+        }
+        store(vw, sm + C::OFF_V + st * C::BYTES);
+        sk *= kmul;
+        scale_s[st * 256 + dt] = sk;
         scale_s[st * 256 + 128 + dt] = sv;
-        // largest V scale of the tile (bits order like the values; a NaN does not count)
-        const uint32_t b = __float_as_uint(sv) & 0x7fffffffu;
-        const uint32_t mx = __reduce_max_sync(0xffffffffu, b > 0x7f800000u ? 0u : b);
-        if (lane == 0) svm_s[st][dw] = mx;
-        store(nxt, sm + C::OFF_V + st * C::BYTES);
+        // largest scales of 32 keys (bits order like the values; a NaN does not count)
+        const uint32_t kb = __float_as_uint(sk) & 0x7fffffffu, vb = __float_as_uint(sv) & 0x7fffffffu;
+        const uint32_t km = __reduce_max_sync(0xffffffffu, kb > 0x7f800000u ? 0u : kb);
+        const uint32_t vm = __reduce_max_sync(0xffffffffu, vb > 0x7f800000u ? 0u : vb);
         __syncwarp();
-        if (lane == 0) ck_arrive(&v_full[st]);
-        pages = next_pages;
-      }
-    }
-  } else if (warp == CK_MMA) {
-    // ======== every MMA. Step j of a segment: softmax group j & 1, key tile
-    // j (alternating) or j / 2; S of step j + 2 follows P V of step j.
-    if (lane == 0) {
-      constexpr uint32_t ID_S = ck_idesc(128, false), ID_O = ck_idesc(HD, true);
-      const uint32_t sb = smem_u32(sm);
-      unsigned fill = 0, seg = 0, np[2] = {0, 0};
-      bool dead = false;
-      for (unsigned u = u0; u < u1 && !dead; ++seg) {
-        CkSeg x;
-        u = segment(u, x);
-        const int nt = x.hi - x.lo, J = x.alt ? nt : 2 * nt;
-        if (!mbar_wait_bounded(&q_full, seg & 1, a.spin) || *abort_v) {
-          give_up();
-          break;
+        if (lane == 0) {
+          skm_s[st][dw] = km;
+          svm_s[st][dw] = vm;
+          ck_arrive(&v_full[st]);
         }
-        ck_fence_after();
-        auto scores = [&](int j) {
-          const int t = j & 1, kt = x.alt ? j : j >> 1;
-          const unsigned f = fill + kt;
-          const int st = f & 1;
-          if (!mbar_wait_bounded(&k_full[st], (f >> 1) & 1, a.spin) || *abort_v) return false;
-          ck_fence_after();
-          const uint32_t ka = sb + C::OFF_K + st * C::BYTES;
-          const uint32_t qa = sb + (F32 || x.alt ? 0 : t * C::BYTES);
-          const uint32_t d = tmem + CK_S + t * 128;
-#pragma unroll
-          for (int part = 0; part < (F32 ? 2 : 1); ++part)  // fp32 rows: lo, then hi
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-              const uint32_t o = (kk >> 2) * CK_TILE + (kk & 3) * 32;
-              ck_mma_ss(d, ck_desc(qa + (F32 ? (1 - part) * C::BYTES : 0) + o, 16), ck_desc(ka + o, 16), ID_S, (part | kk) != 0);
-            }
-          ck_commit(&s_full[t]);
-          if (x.alt || t == 1) ck_commit(&k_empty[st]);
-          return true;
-        };
-        for (int j = 0; j < 2 && j < J && !dead; ++j) dead = !scores(j);
-        for (int j = 0; j < J && !dead; ++j) {
-          const int t = j & 1, kt = x.alt ? j : j >> 1;
-          const unsigned f = fill + kt;
-          const int st = f & 1;
-          if (!mbar_wait_bounded(&v_full[st], (f >> 1) & 1, a.spin) || !mbar_wait_bounded(&p_full[t], np[t] & 1, a.spin) || *abort_v) {
-            dead = true;
-            break;
-          }
-          ++np[t];
-          ck_fence_after();
-          const uint32_t va = sb + C::OFF_V + st * C::BYTES;
-          const uint32_t d = tmem + CK_O + t * 128, p = tmem + CK_S + t * 128;
-          const int fresh = x.alt ? j < 2 : kt == 0;  // this group's first tile: O starts here
-#pragma unroll
-          for (int part = 0; part < (F32 ? 2 : 1); ++part)
-#pragma unroll
-            for (int kk = 0; kk < CK_KEYS / 16; ++kk)
-              ck_mma_ts(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + (F32 ? (1 - part) * 16 : 0), ck_desc(va + kk * 2048, CK_TILE), ID_O,
-                        !(fresh && part == 0 && kk == 0));
-          if (x.alt || t == 1) ck_commit(&v_empty[st]);
-          if (j + 2 >= J) ck_commit(&o_full[t]);
-          else dead = !scores(j + 2);
+        if (c + 1 < x.hi) {
+          load(c + 1, p1, true, vw);
+          load_s(c + 1, p1);
         }
-        fill += nt;
+        p1 = p2;
+        p2 = p3;
       }
-      if (dead) give_up();
-      ck_commit(&idle);  // completes once every MMA issued above is done
+      fill += x.hi - x.lo;
     }
-  } else if (warp < CK_DEQ) {
+  } else {
     // ======== softmax: thread = row
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // row of its tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tm = tmem + lanes + CK_S + t * 128, o_tm = tmem + lanes + CK_O + t * 128;
-    unsigned fill = 0, ns = 0, no = 0;
+    unsigned fill = 0, ns = 0, no = 0, nw = 0;
     bool dead = false;
     auto pair_bar = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    auto group_bar = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory"); };
+    // The group's first warp issues its MMAs: the warp walks together and one
+    // elected lane issues, so that descriptors stay in uniform registers (eight
+    // MMAs issue in 70 to 130 cycles where a lone thread took 390; they run
+    // for 515)
+    const bool issuer = (warp & 3) == 0, lead = issuer && ck_elect();
+    constexpr uint32_t ID_S = ck_idesc(128, false), ID_O = ck_idesc(HD, true);
+    const uint32_t sb32 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int tt = __shfl_sync(0xffffffffu, t, 0);
     for (unsigned u = u0; u < u1;) {
       CkSeg x;
       const unsigned un = segment(u, x);
@@ -525,8 +547,6 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
           if constexpr (F32) *reinterpret_cast<uint4*>(at + C::BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) ck_arrive(&q_full);
       }
       const float slope = a.slopes && ok ? __ldg(a.slopes + head) * KVQ_LOG2E : 0.f;
       // keys that every row of the block sees; this row's own limits
@@ -536,108 +556,221 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
       float m = -INFINITY, l = 0.f, ref = 0.f;
       int ev = -100;
       const int J = x.alt ? nt : 2 * nt;
-      for (int j = t; j < J && !dead; j += 2, ++ns) {
+      ck_fence_before();
+      pair_bar();  // Q is in shared memory
+      // S of step j: this group's row tile, key tile j (alternating) or j / 2
+      auto ask_s = [&](int j) {
+        const unsigned f = fill + (x.alt ? j : j >> 1);
+        const int st = f & 1;
+        if (!wait(&k_full[st], f >> 1)) return false;
+        ck_fence_after();
+        if (lead) {
+          const uint64_t kd = ck_desc(sb32 + C::OFF_K + st * C::BYTES, 16);
+          const uint64_t qd = ck_desc(sb32 + (F32 || x.alt ? 0 : tt * C::BYTES), 16);
+          const uint32_t d = tm + CK_S + tt * 128;
+#pragma unroll
+          for (int part = 0; part < (F32 ? 2 : 1); ++part)  // fp32 rows: lo, then hi
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * CK_TILE + (kk & 3) * 32) >> 4;
+              ck_mma_ss(d, qd + (F32 ? (1 - part) * C::BYTES >> 4 : 0) + o, kd + o, ID_S, (part | kk) != 0);
+            }
+          ck_commit(&s_full[tt]);
+          ck_commit(&k_empty[st]);
+          if (x.alt) ck_commit(&k_empty[st]);
+        }
+        __syncwarp();
+        return true;
+      };
+      if (issuer && t < J && !dead) dead = !ask_s(t);
+      // a warp that gave up keeps the group's barriers and skips the rest
+      for (int j = t; j < J; j += 2, ++ns) {
         const int kt = x.alt ? j : j >> 1, j0 = x.key(x.lo + kt);
         const unsigned f = fill + kt;
         const int st = f & 1;
-        if (!wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns)) {
-          dead = true;
-          break;
-        }
-        ck_fence_after();
-        const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
-        const float4* vsc = ksc + 32;
-        const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
-        // x of columns 32 c .. 32 c + 31
-        auto scores = [&](int c, float (&z)[32]) {
-          ck_ld32(s_tm + 32 * c, z);
+        if (!dead) dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns);
+        if (!dead) {
+          ck_fence_after();
+          const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
+          const float4* vsc = ksc + 32;
+          const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
+          // x of columns 32 c .. 32 c + 31
+          auto scores = [&](int c, float (&z)[32]) {
+            ck_get32(s_tm + 32 * c, z);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 k4 = ksc[8 * c + i];
-            if constexpr (F32) {
-              z[4 * i] *= k4.x * rmul; z[4 * i + 1] *= k4.y * rmul; z[4 * i + 2] *= k4.z * rmul; z[4 * i + 3] *= k4.w * rmul;
-            } else {
-              z[4 * i] *= k4.x; z[4 * i + 1] *= k4.y; z[4 * i + 2] *= k4.z; z[4 * i + 3] *= k4.w;
+            for (int i = 0; i < 8; ++i) {
+              const float4 k4 = ksc[8 * c + i];
+              const float k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) z[4 * i + e] *= F32 ? k[e] * rmul : k[e];
             }
-          }
-          if (a.cap > 0.f) {
+            if (!PLAIN && a.cap > 0.f) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
-          }
-          if (a.slopes) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + 32 * c + i))), z[i]);
-          }
-          if (!inner) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int k = j0 + 32 * c + i;
-              if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
+              for (int i = 0; i < 32; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
             }
-          }
-        };
-        float mx = -INFINITY;
+            if (!PLAIN && a.slopes) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + 32 * c + i))), z[i]);
+            }
+            if (!inner) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const int k = j0 + 32 * c + i;
+                if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
+              }
+            }
+          };
+          // Does the reference hold? The common tile (no cap, no bias, nothing
+          // masked) asks a bound first, the largest raw product of 32 keys times
+          // their largest K scale, which needs no key's own scale.
+          const bool fast = PLAIN && inner;
+          const int en = max(ev, min(100, (int)(max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3])) >> 23) - 126));
+          float mx = m;
+          if (fast) {
+            float z[2][32];
+            ck_ld32(s_tm, z[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              ck_wait_ld(z[c & 1]);
+              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[(c + 1) & 1]);
+              float(&w)[32] = z[c & 1];
+              float top[2] = {0.f, 0.f};
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                top[0] = fmaxf(top[0], fmaxf(w[i], w[i + 1]));
+                top[1] = fmaxf(top[1], fmaxf(w[i + 2], w[i + 3]));
+              }
+              if (__any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) * (__uint_as_float(skm_s[st][c]) * rmul) <= m + CkLift<F32>::MARGIN))) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 k4 = ksc[8 * c + i];
+                  const float e0 = fmaxf(w[4 * i] * k4.x, w[4 * i + 1] * k4.y), e1 = fmaxf(w[4 * i + 2] * k4.z, w[4 * i + 3] * k4.w);
+                  mx = fmaxf(mx, fmaxf(e0, e1) * rmul);
+                }
+              }
+            }
+          } else {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float z[32];
-          scores(c, z);
+            for (int c = 0; c < 4; ++c) {
+              float z[32];
+              scores(c, z);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, z[i]);
-        }
-        // a score past the maximum by 2^8, or a V scale past 2^ev
-        const uint32_t sb = max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3]));
-        const int en = max(ev, min(100, (int)(sb >> 23) - 126));
-        if (__any_sync(0xffffffffu, mx > m + 8.f || en > ev)) {
-          const float mn = fmaxf(m, mx);
-          const float rn = (mn == -INFINITY ? 0.f : mn) - 7.f + (float)en;
-          const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
-          m = mn;
-          ev = en;
-          ref = rn;
-          l *= fac;
-          if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
-#pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              float o[32];
-              ck_ld32(o_tm + 32 * c, o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= fac;
-              ck_st32(o_tm + 32 * c, o);
+              for (int i = 0; i < 32; ++i) mx = fmaxf(mx, z[i]);
             }
           }
-        }
+          if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
+            const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT + (float)en;
+            const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
+            m = mx;
+            ev = en;
+            ref = rn;
+            l *= fac;
+            if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float z[32];
-          scores(c, z);
-          uint32_t ph[16], pl[F32 ? 16 : 1];
+              for (int c = 0; c < HD / 32; ++c) {
+                float o[32];
+                ck_get32(o_tm + 32 * c, o);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 v4 = vsc[8 * c + i];
-            const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = ex2(z[4 * i + e] - ref);
-              l += y;
-              p[e] = y * vs[e];
-              if (!inner && y == 0.f) p[e] = 0.f;  // a masked key counts for nothing, whatever its scale holds
-            }
-            if constexpr (F32) {
-              ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
-              ph[2 * i + 1] = split_h2(p[2], p[3], pl[2 * i + 1]);
-            } else {
-              ph[2 * i] = half2_bits(__floats2half2_rn(p[0], p[1]));
-              ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
+                for (int i = 0; i < 32; ++i) o[i] *= fac;
+                ck_st32(o_tm + 32 * c, o);
+              }
             }
           }
-          ck_st16(s_tm + 32 * c, ph);
-          if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
+          if (fast) {
+            float z[2][32];
+            ck_ld32(s_tm, z[0]);
+            const float2 nref = make_float2(-ref, -ref);
+            float2 l2[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              ck_wait_ld(z[c & 1]);
+              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[(c + 1) & 1]);
+              float(&w)[32] = z[c & 1];
+              uint32_t ph[16], pl[F32 ? 16 : 1];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 k4 = ksc[8 * c + i], v4 = vsc[8 * c + i];
+                float2 u0 = make_float2(w[4 * i], w[4 * i + 1]), u1 = make_float2(w[4 * i + 2], w[4 * i + 3]);
+                if constexpr (F32) {
+                  u0 = mul2(u0, make_float2(rmul, rmul));
+                  u1 = mul2(u1, make_float2(rmul, rmul));
+                }
+                u0 = fma2(u0, make_float2(k4.x, k4.y), nref);
+                u1 = fma2(u1, make_float2(k4.z, k4.w), nref);
+                u0.x = ex2(u0.x); u0.y = ex2(u0.y); u1.x = ex2(u1.x); u1.y = ex2(u1.y);
+                l2[0] = add2(l2[0], u0);
+                l2[1] = add2(l2[1], u1);
+                u0 = mul2(u0, make_float2(v4.x, v4.y));
+                u1 = mul2(u1, make_float2(v4.z, v4.w));
+                if constexpr (F32) {
+                  ph[2 * i] = split_h2(u0.x, u0.y, pl[2 * i]);
+                  ph[2 * i + 1] = split_h2(u1.x, u1.y, pl[2 * i + 1]);
+                } else {
+                  ph[2 * i] = half2_bits(__floats2half2_rn(u0.x, u0.y));
+                  ph[2 * i + 1] = half2_bits(__floats2half2_rn(u1.x, u1.y));
+                }
+              }
+              ck_st16(s_tm + 32 * c, ph);
+              if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
+            }
+            l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float z[32];
+              scores(c, z);
+              uint32_t ph[16], pl[F32 ? 16 : 1];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 v4 = vsc[8 * c + i];
+                const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float y = ex2(z[4 * i + e] - ref);
+                  l += y;
+                  p[e] = y == 0.f ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
+                }
+                if constexpr (F32) {
+                  ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
+                  ph[2 * i + 1] = split_h2(p[2], p[3], pl[2 * i + 1]);
+                } else {
+                  ph[2 * i] = half2_bits(__floats2half2_rn(p[0], p[1]));
+                  ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
+                }
+              }
+              ck_st16(s_tm + 32 * c, ph);
+              if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
+            }
+          }
+          ck_wait_st();
+          ck_fence_before();
         }
-        ck_wait_st();
-        ck_fence_before();
-        __syncwarp();
-        if (lane == 0) ck_arrive(&p_full[t]);
+        group_bar();  // the group's P (and rescaled O) is complete
+        // The groups issue in turn, P V and the next S together: their tiles
+        // then run on the tensor pipe one after the other, and one group
+        // exponentiates while the other's run (left alone both fall into step).
+        if (issuer && !dead) {
+          if (j > 0) dead = !wait(&turn[t], nw++);
+          ck_fence_after();
+          if (lead && !dead) {
+            const uint64_t vd = ck_desc(sb32 + C::OFF_V + st * C::BYTES, CK_TILE);
+            const uint32_t d = tm + CK_O + tt * 128, p = tm + CK_S + tt * 128;
+            const int fresh = j < 2;  // this group's first tile: O starts here
+#pragma unroll
+            for (int part = 0; part < (F32 ? 2 : 1); ++part)
+#pragma unroll
+              for (int kk = 0; kk < CK_KEYS / 16; ++kk)
+                ck_mma_ts(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + (F32 ? (1 - part) * 16 : 0), vd + kk * (2048 >> 4), ID_O,
+                          (part | kk) != 0 || !fresh);
+            ck_commit(&v_empty[st]);
+            if (x.alt) ck_commit(&v_empty[st]);
+            if (j + 2 >= J) ck_commit(&o_full[tt]);
+          }
+          __syncwarp();
+          if (!dead && j + 2 < J) dead = !ask_s(j + 2);
+          if (lane == 0 && j + 1 < J) ck_arrive(&turn[t ^ 1]);
+        }
       }
       fill += nt;
 
@@ -662,7 +795,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
               float o[32];
-              ck_ld32(o_tm + 32 * c, o);
+              ck_get32(o_tm + 32 * c, o);
 #pragma unroll
               for (int i = 0; i < 8; ++i) *at(row, 8 * c + i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             }
@@ -708,7 +841,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           float o[32];
-          ck_ld32(o_tm + 32 * c, o);
+          ck_get32(o_tm + 32 * c, o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = f1 == 0.f && L == L ? 0.f : o[i] * f1;
           if (other) {
@@ -786,10 +919,11 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
       }
       u = un;
     }
+    if (lead) ck_commit(&idle);  // completes once every MMA this lane issued is done
   }
   ck_fence_before();
   __syncthreads();
-  if (warp == CK_MMA) {
+  if (warp == 0) {
     if (lane == 0) mbar_wait_bounded(&idle, 0u, MBAR_SPIN_LIMIT);  // no MMA may still write the memory that is freed
     __syncwarp();
     ck_fence_after();
@@ -802,7 +936,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
 template <int HD, int BITS, typename T>
 int kvq_chunk_launch(AttendArgs a, cudaStream_t s) {
   using C = CkCfg<HD>;
-  auto kern = kvq_chunk_kernel<HD, BITS, T>;
+  auto kern = a.cap > 0.f || a.slopes ? kvq_chunk_kernel<HD, BITS, T, false> : kvq_chunk_kernel<HD, BITS, T, true>;
   a.min_cells = 2;
   const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_chunk");
   if (rc) return rc;
