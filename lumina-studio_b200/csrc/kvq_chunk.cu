@@ -167,6 +167,31 @@ __device__ __forceinline__ bool ck_elect() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
   return r != 0;
 }
+__device__ __forceinline__ void ck_ld8(uint32_t addr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = __uint_as_float(r[i]);
+    asm volatile("" : "+f"(v[i]));
+  }
+}
+template <int N>
+__device__ __forceinline__ void ck_get(uint32_t addr, float (&v)[N]) {
+  if constexpr (N == 32) ck_get32(addr, v);
+  else ck_ld8(addr, v);
+}
+template <int N>
+__device__ __forceinline__ void ck_put(uint32_t addr, const uint32_t (&r)[N]) {
+  if constexpr (N == 16)
+    ck_st16(addr, r);
+  else
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 __device__ __forceinline__ void ck_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One segment: key tiles [lo, hi) of one task.
@@ -179,8 +204,68 @@ struct CkSeg {
   __device__ __forceinline__ int key(int c) const { return (c < tp ? c : c - tp + tl) * CK_KEYS; }
 };
 
+// The line of units as a CTA sees it.
+struct CkLine {
+  const AttendArgs& a;
+  const int *line, *blocks;
+  int NBt, Tn;
+  unsigned share, u0, u1;
+  bool whole;
+};
+
+// task b of the block line (any KV head): everything but kvh, lo, hi
+template <int BM>
+__device__ __noinline__ void ck_describe(const CkLine& ln, int b, CkSeg& x) {
+  const AttendArgs& a = ln.a;
+  const KvqView& v = a.v;
+  int lo = 0, hi = v.n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ln.blocks[mid] > b) hi = mid;
+    else lo = mid + 1;
+  }
+  x.s = lo;
+  x.n = kvq_seq_rows(v, lo, x.first, false);
+  x.len = min(v.pages_ld << v.page_shift, max(0, __ldg(v.len + lo)));
+  x.pre = a.prefix ? min(x.len, max(0, __ldg(a.prefix + lo))) : 0;
+  x.row0 = (b - (lo ? ln.blocks[lo - 1] : 0)) * BM;
+  x.rows = min(BM, x.n * a.G - x.row0);
+  x.alt = x.rows <= 128;
+  const int p0 = x.len - x.n, p_lo = p0 + x.row0 / a.G, p_hi = p0 + (x.row0 + x.rows - 1) / a.G;
+  const int k_hi = min(x.len, max(0, p_hi + 1)), k_lo = a.window ? min(k_hi, max(0, p_lo - a.window + 1)) : 0;
+  x.tp = (x.pre + CK_KEYS - 1) / CK_KEYS;
+  x.tl = max(x.tp, k_lo / CK_KEYS);
+  x.total = max(1, x.tp + max(x.tl, (k_hi + CK_KEYS - 1) / CK_KEYS) - x.tl);
+}
+
+// the segment that starts at unit u; returns the next segment's unit. Out of
+// line: once per segment, and the loops that call it have to fit the
+// instruction cache.
+template <int BM>
+__device__ __noinline__ unsigned ck_segment(const CkLine& ln, unsigned u, CkSeg& x) {
+  const int kvh = u / ln.Tn, c = u - kvh * ln.Tn;
+  if (ln.whole) {
+    ck_describe<BM>(ln, c, x);
+    x.kvh = kvh;
+    x.lo = 0;
+    x.hi = x.total;
+    return u + gridDim.x;
+  }
+  int lo = 0, hi = ln.NBt - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ln.line[mid] > c) hi = mid;
+    else lo = mid + 1;
+  }
+  ck_describe<BM>(ln, lo, x);
+  x.kvh = kvh;
+  x.lo = c - (lo ? ln.line[lo - 1] : 0);
+  x.hi = (int)min((unsigned)x.total, x.lo + (ln.u1 - u));
+  return u + (unsigned)(x.hi - x.lo);
+}
+
 template <int HD, int BITS, typename T, bool PLAIN>
-__global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_constant__ AttendArgs a) {
   using C = CkCfg<HD>;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int BM = F32 ? 128 : 256;                    // packed rows of a block
@@ -251,28 +336,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
     NBt += total;
   }
   __syncthreads();
-  // task b of the block line (any KV head): everything but kvh, lo, hi
-  auto describe = [&](int b, CkSeg& x) {
-    int lo = 0, hi = v.n_seq - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (blocks[mid] > b) hi = mid;
-      else lo = mid + 1;
-    }
-    x.s = lo;
-    x.n = kvq_seq_rows(v, lo, x.first, false);
-    x.len = min(cap_tokens, max(0, __ldg(v.len + lo)));
-    x.pre = a.prefix ? min(x.len, max(0, __ldg(a.prefix + lo))) : 0;
-    x.row0 = (b - (lo ? blocks[lo - 1] : 0)) * BM;
-    x.rows = min(BM, x.n * a.G - x.row0);
-    x.alt = x.rows <= 128;
-    const int p0 = x.len - x.n, p_lo = p0 + x.row0 / a.G, p_hi = p0 + (x.row0 + x.rows - 1) / a.G;
-    const int k_hi = min(x.len, max(0, p_hi + 1)), k_lo = a.window ? min(k_hi, max(0, p_lo - a.window + 1)) : 0;
-    x.tp = (x.pre + CK_KEYS - 1) / CK_KEYS;
-    x.tl = max(x.tp, k_lo / CK_KEYS);
-    x.total = max(1, x.tp + max(x.tl, (k_hi + CK_KEYS - 1) / CK_KEYS) - x.tl);
-  };
-  const bool whole = NBt > KVQ_MAX_BLOCKS;  // whole tasks: the line does not hold them
+  CkLine ln{a, line, blocks, 0, 0, 0u, 0u, 0u, false};
+  ln.NBt = NBt;
+  const bool whole = ln.whole = NBt > KVQ_MAX_BLOCKS;  // whole tasks: the line does not hold them
   int Tn = NBt;                             // units of one KV head: tiles, or tasks
   if (!whole) {
     Tn = 0;
@@ -280,7 +346,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
       CkSeg x;
       x.total = 0;
       int total;
-      if (b0 + tid < NBt) describe(b0 + tid, x);
+      if (b0 + tid < NBt) ck_describe<BM>(ln, b0 + tid, x);
       const int inc = block_scan(x.total, total);
       if (b0 + tid < NBt) line[b0 + tid] = Tn + inc;
       Tn += total;
@@ -296,39 +362,26 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
   const unsigned share = whole ? 1u : max((U + gridDim.x - 1) / gridDim.x, (unsigned)a.min_cells);
   // units [u0, u1), or tasks u0, u0 + gridDim.x, ...
   const unsigned u0 = whole ? blockIdx.x : min(U, blockIdx.x * share), u1 = whole ? U : min(U, u0 + share);
-  auto segment = [&](unsigned u, CkSeg& x) {  // returns the next segment's unit
-    x.kvh = u / Tn;
-    const int c = u - x.kvh * Tn;
-    if (whole) {
-      describe(c, x);
-      x.lo = 0;
-      x.hi = x.total;
-      return u + gridDim.x;
-    }
-    int lo = 0, hi = NBt - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (line[mid] > c) hi = mid;
-      else lo = mid + 1;
-    }
-    describe(lo, x);
-    x.lo = c - (lo ? line[lo - 1] : 0);
-    x.hi = (int)min((unsigned)x.total, x.lo + (u1 - u));
-    return u + (unsigned)(x.hi - x.lo);
-  };
+  ln.Tn = Tn;
+  ln.share = share;
+  ln.u0 = u0;
+  ln.u1 = u1;
+  auto segment = [&](unsigned u, CkSeg& x) { return ck_segment<BM>(ln, u, x); };  // returns the next segment's unit
   auto give_up = [&]() {
     if (!*abort_v) kvq_fault(v, KVQ_FAULT_WAIT);
     *abort_v = 1;
   };
+  const unsigned spin = (unsigned)min(a.spin, 0x7fffffffLL);
   // a whole warp waits; false when this wait or, meanwhile, any role gave up
   auto wait = [&](uint64_t* bar, unsigned phase) {
     bool in = false;
-    for (long long i = 0; i < a.spin; ++i) {
+#pragma unroll 1
+    for (unsigned i = 0; i < spin; ++i) {
       if (mbar_try_wait(bar, phase & 1)) {
         in = true;
         break;
       }
-      if ((i & 1023) == 1023 && *abort_v) break;
+      if ((i & 1023u) == 1023u && *abort_v) break;
     }
     in = __all_sync(0xffffffffu, in);
     if (!in && lane == 0) give_up();
@@ -402,69 +455,60 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       };
       // order: K 0, K 1, V 0, K 2, V 1, ...: S of a tile is wanted before P V
-      // of the one before it. Codes and scales are in registers a tile ahead
-      // of their store, page numbers a tile ahead of that.
-      const int p0 = ask(x.lo);
-      int p1 = ask(x.lo + 1), p2 = ask(x.lo + 2);  // pages of tiles c + 1, c + 2
-      uint4 kw[NP], vw[NP];
-      float sk, sv;
-      auto load_s = [&](int c, int pages) {  // tile c's scales (thread = key)
-        const int j = x.key(c) + dt;
-        const int pg = __shfl_sync(0xffffffffu, pages, dt >> 4);
-        const bool there = j < x.len && (unsigned)pg < (unsigned)v.n_pages;
-        if (j < x.len && !there && pg != -2) kvq_fault(v, KVQ_FAULT_DATA);
-        sk = sv = 0.f;
-        if (there && (j >= win_any || j < x.pre)) {
-          const float* sc = reinterpret_cast<const float*>(base + (size_t)pg * v.page_bytes + 2 * P * NB) + (j & (P - 1));
-          sk = __ldg(sc);
-          sv = __ldg(sc + P);
-        }
+      // of the one before it. A step's codes (and scales) are asked for when
+      // the step before is stored, its page numbers a step earlier.
+      const int nt = x.hi - x.lo;
+      auto after = [&](int s) {  // steps are 2 * tile + (V ? 1 : 0); 2 nt: the end
+        const int c = s >> 1;
+        if (s & 1) return c + 2 < nt ? s + 3 : s + 2 < 2 * nt ? s + 2 : 2 * nt;
+        return c == 0 ? (nt > 1 ? 2 : 1) : s - 1;
       };
-      load(x.lo, p0, false, kw);
-      load(x.lo, p0, true, vw);
-      load_s(x.lo, p0);
-      auto fill_k = [&](int c, int next_pages) {
-        const unsigned f = fill + (c - x.lo);
-        if (f >= 2 && !wait(&k_empty[f & 1], (f >> 1) + 1)) return false;
-        store(kw, sm + C::OFF_K + (f & 1) * C::BYTES);
-        __syncwarp();
-        if (lane == 0) ck_arrive(&k_full[f & 1]);
-        if (c + 1 < x.hi) load(c + 1, next_pages, false, kw);
-        return true;
-      };
-      dead = !fill_k(x.lo, p1);
-      for (int c = x.lo; c < x.hi && !dead; ++c) {
-        const int p3 = ask(c + 3);
-        if (c + 1 < x.hi && !fill_k(c + 1, p2)) {
-          dead = true;
-          break;
+      uint4 w[NP];
+      float sk = 0.f, sv = 0.f;
+      int s0 = -1, s1 = 0, pg1 = ask(x.lo);  // the step in registers, the next one and its pages
+#pragma unroll 1
+      while (true) {
+        if (s0 >= 0) {
+          const unsigned f = fill + (s0 >> 1);
+          const int st = f & 1;
+          if (f >= 2 && !wait((s0 & 1 ? v_empty : k_empty) + st, (f >> 1) + 1)) {
+            dead = true;
+            break;
+          }
+          store(w, sm + (s0 & 1 ? C::OFF_V : C::OFF_K) + st * C::BYTES);
+          if (s0 & 1) {
+            scale_s[st * 256 + dt] = sk;
+            scale_s[st * 256 + 128 + dt] = sv;
+            // largest scales of 32 keys (bits order like the values; a NaN does not count)
+            const uint32_t kb = __float_as_uint(sk) & 0x7fffffffu, vb = __float_as_uint(sv) & 0x7fffffffu;
+            const uint32_t km = __reduce_max_sync(0xffffffffu, kb > 0x7f800000u ? 0u : kb);
+            const uint32_t vm = __reduce_max_sync(0xffffffffu, vb > 0x7f800000u ? 0u : vb);
+            if (lane == 0) {
+              skm_s[st][dw] = km;
+              svm_s[st][dw] = vm;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) ck_arrive((s0 & 1 ? v_full : k_full) + st);
         }
-        const unsigned f = fill + (c - x.lo);
-        const int st = f & 1;
-        if (f >= 2 && !wait(&v_empty[st], (f >> 1) + 1)) {
-          dead = true;
-          break;
+        if (s1 >= 2 * nt) break;
+        load(x.lo + (s1 >> 1), pg1, s1 & 1, w);
+        if (s1 & 1) {  // the tile's scales (thread = key)
+          const int j = x.key(x.lo + (s1 >> 1)) + dt;
+          const int pg = __shfl_sync(0xffffffffu, pg1, dt >> 4);
+          const bool there = j < x.len && (unsigned)pg < (unsigned)v.n_pages;
+          if (j < x.len && !there && pg != -2) kvq_fault(v, KVQ_FAULT_DATA);
+          sk = sv = 0.f;
+          if (there && (j >= win_any || j < x.pre)) {
+            const float* sc = reinterpret_cast<const float*>(base + (size_t)pg * v.page_bytes + 2 * P * NB) + (j & (P - 1));
+            sk = __ldg(sc);
+            sv = __ldg(sc + P);
+          }
+          sk *= kmul;
         }
-        store(vw, sm + C::OFF_V + st * C::BYTES);
-        sk *= kmul;
-        scale_s[st * 256 + dt] = sk;
-        scale_s[st * 256 + 128 + dt] = sv;
-        // largest scales of 32 keys (bits order like the values; a NaN does not count)
-        const uint32_t kb = __float_as_uint(sk) & 0x7fffffffu, vb = __float_as_uint(sv) & 0x7fffffffu;
-        const uint32_t km = __reduce_max_sync(0xffffffffu, kb > 0x7f800000u ? 0u : kb);
-        const uint32_t vm = __reduce_max_sync(0xffffffffu, vb > 0x7f800000u ? 0u : vb);
-        __syncwarp();
-        if (lane == 0) {
-          skm_s[st][dw] = km;
-          svm_s[st][dw] = vm;
-          ck_arrive(&v_full[st]);
-        }
-        if (c + 1 < x.hi) {
-          load(c + 1, p1, true, vw);
-          load_s(c + 1, p1);
-        }
-        p1 = p2;
-        p2 = p3;
+        s0 = s1;
+        s1 = after(s1);
+        pg1 = ask(x.lo + (s1 >> 1));
       }
       fill += x.hi - x.lo;
     }
@@ -582,40 +626,43 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
         __syncwarp();
         return true;
       };
-      if (issuer && t < J && !dead) dead = !ask_s(t);
-      // a warp that gave up keeps the group's barriers and skips the rest
-      for (int j = t; j < J; j += 2, ++ns) {
+      // a warp that gave up keeps the group's barriers and skips the rest;
+      // step t - 2 only asks for the first S
+#pragma unroll 1
+      for (int j = t - 2; j < J; j += 2) {
         const int kt = x.alt ? j : j >> 1, j0 = x.key(x.lo + kt);
         const unsigned f = fill + kt;
         const int st = f & 1;
-        if (!dead) dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns);
-        if (!dead) {
+        if (j >= 0 && !dead) dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns++);
+        if (j >= 0 && !dead) {
           ck_fence_after();
           const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
           const float4* vsc = ksc + 32;
           const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
-          // x of columns 32 c .. 32 c + 31
-          auto scores = [&](int c, float (&z)[32]) {
-            ck_get32(s_tm + 32 * c, z);
+          // x of columns GC c .. GC c + GC - 1; where the common tile has its own
+          // code this one is kept small
+          constexpr int GC = PLAIN && !F32 ? 8 : 32;  // (fp32 rows' low parts go to columns that have to be read first)
+          auto scores = [&](int c, float (&z)[GC]) {
+            ck_get<GC>(s_tm + GC * c, z);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 k4 = ksc[8 * c + i];
+            for (int i = 0; i < GC / 4; ++i) {
+              const float4 k4 = ksc[GC / 4 * c + i];
               const float k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) z[4 * i + e] *= F32 ? k[e] * rmul : k[e];
             }
             if (!PLAIN && a.cap > 0.f) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
+              for (int i = 0; i < GC; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
             }
             if (!PLAIN && a.slopes) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + 32 * c + i))), z[i]);
+              for (int i = 0; i < GC; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + GC * c + i))), z[i]);
             }
             if (!inner) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const int k = j0 + 32 * c + i;
+              for (int i = 0; i < GC; ++i) {
+                const int k = j0 + GC * c + i;
                 if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
               }
             }
@@ -629,11 +676,14 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
           if (fast) {
             float z[2][32];
             ck_ld32(s_tm, z[0]);
+#pragma unroll 1
+            for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              ck_wait_ld(z[c & 1]);
-              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[(c + 1) & 1]);
-              float(&w)[32] = z[c & 1];
+            for (int h = 0; h < 2; ++h) {
+              const int c = c2 + h;
+              ck_wait_ld(z[h]);
+              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
+              float(&w)[32] = z[h];
               float top[2] = {0.f, 0.f};
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -651,11 +701,11 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
             }
           } else {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              float z[32];
+            for (int c = 0; c < 128 / GC; ++c) {
+              float z[GC];
               scores(c, z);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) mx = fmaxf(mx, z[i]);
+              for (int i = 0; i < GC; ++i) mx = fmaxf(mx, z[i]);
             }
           }
           if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
@@ -681,11 +731,14 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
             ck_ld32(s_tm, z[0]);
             const float2 nref = make_float2(-ref, -ref);
             float2 l2[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+            for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              ck_wait_ld(z[c & 1]);
-              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[(c + 1) & 1]);
-              float(&w)[32] = z[c & 1];
+            for (int h = 0; h < 2; ++h) {
+              const int c = c2 + h;
+              ck_wait_ld(z[h]);
+              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
+              float(&w)[32] = z[h];
               uint32_t ph[16], pl[F32 ? 16 : 1];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -716,13 +769,13 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
             l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
           } else {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              float z[32];
+            for (int c = 0; c < 128 / GC; ++c) {
+              float z[GC];
               scores(c, z);
-              uint32_t ph[16], pl[F32 ? 16 : 1];
+              uint32_t ph[GC / 2], pl[F32 ? GC / 2 : 1];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 v4 = vsc[8 * c + i];
+              for (int i = 0; i < GC / 4; ++i) {
+                const float4 v4 = vsc[GC / 4 * c + i];
                 const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
                 float p[4];
 #pragma unroll
@@ -739,21 +792,25 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
                   ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
                 }
               }
-              ck_st16(s_tm + 32 * c, ph);
-              if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
+              // keys 32 k ..: 16 columns of pairs at 32 k (and 16 of low parts).
+              // GC = 8 overwrites columns 32 k + 4 r ..: of chunk r = 0 the first
+              // four of its own, later ones columns that were read before.
+              const uint32_t to = s_tm + (GC * c & ~31) + (GC * c & 31) / 2;
+              ck_put<GC / 2>(to, ph);
+              if constexpr (F32) ck_put<GC / 2>(to + 16, pl);
             }
           }
           ck_wait_st();
           ck_fence_before();
         }
-        group_bar();  // the group's P (and rescaled O) is complete
+        if (j >= 0) group_bar();  // the group's P (and rescaled O) is complete
         // The groups issue in turn, P V and the next S together: their tiles
         // then run on the tensor pipe one after the other, and one group
         // exponentiates while the other's run (left alone both fall into step).
         if (issuer && !dead) {
           if (j > 0) dead = !wait(&turn[t], nw++);
           ck_fence_after();
-          if (lead && !dead) {
+          if (lead && !dead && j >= 0) {
             const uint64_t vd = ck_desc(sb32 + C::OFF_V + st * C::BYTES, CK_TILE);
             const uint32_t d = tm + CK_O + tt * 128, p = tm + CK_S + tt * 128;
             const int fresh = j < 2;  // this group's first tile: O starts here
@@ -769,7 +826,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(AttendArgs a) 
           }
           __syncwarp();
           if (!dead && j + 2 < J) dead = !ask_s(j + 2);
-          if (lane == 0 && j + 1 < J) ck_arrive(&turn[t ^ 1]);
+          if (lane == 0 && j >= 0 && j + 1 < J) ck_arrive(&turn[t ^ 1]);
         }
       }
       fill += nt;
