@@ -12,11 +12,11 @@
 // fp32 rows send Q and P as two fp16 parts (hi + lo, about 22 bits) through
 // the same tiles.
 //
-// One CTA per SM, 12 warps (168 registers a thread):
+// One CTA per SM, 13 warps:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: a thread is a row, so
-//                   maximum and sum need no shuffles; each group's first warp
-//                   issues the group's own MMAs, P V and then the next S
+//                   maximum and sum need no shuffles
 //   warps 8-11      codes from global memory to fp16 tiles (128-byte swizzle)
+//   warp 12         issues every MMA, owns the tensor memory
 // The two row tiles take turns on the tensor pipe: while one's S is being
 // exponentiated the other's products run. With at most 128 packed rows (and
 // always for fp32 rows) both softmax groups hold the SAME rows and take
@@ -45,8 +45,8 @@ namespace lumina {
 namespace {
 
 constexpr int CK_KEYS = 128;                // keys per tile
-constexpr int CK_DEQ = 8;                   // first warp that fills tiles
-constexpr int CK_THREADS = 384;
+constexpr int CK_DEQ = 8, CK_MMA = 12;      // first warp of the roles
+constexpr int CK_THREADS = 32 * (CK_MMA + 1);
 // P is 2^LIFT at the maximum the reference was set by, and may grow to 2^15
 // (fp16's range) before the reference moves. fp32 rows need their small p's
 // low parts above fp16's subnormals, fp16 rows a rarely moving reference.
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   float* scale_s = reinterpret_cast<float*>(sm + C::OFF_SC);
   int* line = reinterpret_cast<int*>(sm + C::OFF_LINE);  // inclusive prefix of tiles over blocks
   int* blocks = line + KVQ_MAX_BLOCKS;                   // inclusive prefix of blocks over sequences
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], o_full[2], turn[2], idle;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, idle;
   __shared__ uint32_t tmem_s, skm_s[2][4], svm_s[2][4];  // a tile's largest K and V scale, one per warp that filled it
   __shared__ int scan_s[CK_THREADS / 32], abort_s, last_s;
   __shared__ float m_s[128], l_s[128];
@@ -288,17 +288,18 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&v_full[i], 4);
-      mbar_init(&k_empty[i], 2);  // two commits: one per group, or two of the one that used the stage
-      mbar_init(&v_empty[i], 2);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&turn[i], 1);
+      mbar_init(&p_full[i], 4);
     }
-    mbar_init(&idle, 2);
+    mbar_init(&q_full, 8);
+    mbar_init(&idle, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_s = 0;
   }
-  if (warp == 0) {
+  if (warp == CK_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   };
   const int P = 1 << v.page_shift;
 
-  if (warp >= CK_DEQ) {
+  if (warp >= CK_DEQ && warp < CK_MMA) {
     // ======== codes -> fp16 tiles. A row is LPR 16-byte words of codes, one
     // lane each; a pass of the 128 threads covers 128 / LPR rows.
     constexpr int LPR = NB / 16, RPP = 128 / LPR, NP = LPR;
@@ -512,23 +513,86 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       }
       fill += x.hi - x.lo;
     }
+  } else if (warp == CK_MMA) {
+    // ======== every MMA. Step j of a segment: softmax group j & 1, key tile
+    // j (alternating) or j / 2; S of step j + 2 follows P V of step j, and
+    // the groups' steps alternate, so that one group exponentiates while the
+    // other's products run. The whole warp walks the loop and one elected
+    // lane issues: what is uniform stays in uniform registers, and eight MMAs
+    // issue in 70 to 150 cycles where a lone thread took 390 (they run for 515).
+    constexpr uint32_t ID_S = ck_idesc(128, false), ID_O = ck_idesc(HD, true);
+    const bool lead = ck_elect();
+    const uint32_t sb = __shfl_sync(0xffffffffu, smem_u32(sm), 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    unsigned fill = 0, seg = 0, np0 = 0, np1 = 0;
+    bool dead = false;
+    for (unsigned u = u0; u < u1 && !dead; ++seg) {
+      CkSeg x;
+      u = segment(u, x);
+      const bool alt = x.alt;
+      const int nt = x.hi - x.lo, J = alt ? nt : 2 * nt;
+      dead = !wait(&q_full, seg);
+      // j = -2, -1 only ask for the first S of each group
+#pragma unroll 1
+      for (int j = -2; j < J && !dead; ++j) {
+        const int t = __shfl_sync(0xffffffffu, j & 1, 0);
+        if (j >= 0) {
+          const unsigned f = fill + (alt ? j : j >> 1);
+          const int st = __shfl_sync(0xffffffffu, f & 1, 0);
+          dead = ((alt || t == 0) && !wait(&v_full[st], f >> 1)) || !wait(&p_full[t], t ? np1 : np0);
+          if (dead) break;
+          if (t) ++np1;
+          else ++np0;
+          ck_fence_after();
+          const uint64_t vd = ck_desc(sb + C::OFF_V + st * C::BYTES, CK_TILE);
+          const uint32_t d = tm + CK_O + t * 128, p = tm + CK_S + t * 128;
+          const int fresh = j < 2;  // the group's first tile: O starts here
+          if (lead) {
+#pragma unroll
+            for (int part = 0; part < (F32 ? 2 : 1); ++part)
+#pragma unroll
+              for (int kk = 0; kk < CK_KEYS / 16; ++kk)
+                ck_mma_ts(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + (F32 ? (1 - part) * 16 : 0), vd + kk * (2048 >> 4), ID_O,
+                          (part | kk) != 0 || !fresh);
+            if (alt || t == 1) ck_commit(&v_empty[st]);
+            if (j + 2 >= J) ck_commit(&o_full[t]);
+          }
+          __syncwarp();
+        }
+        if (j + 2 < J) {
+          const unsigned f = fill + (alt ? j + 2 : (j + 2) >> 1);
+          const int st = __shfl_sync(0xffffffffu, f & 1, 0);
+          dead = (alt || t == 0) && !wait(&k_full[st], f >> 1);
+          if (dead) break;
+          ck_fence_after();
+          const uint64_t kd = ck_desc(sb + C::OFF_K + st * C::BYTES, 16);
+          const uint64_t qd = ck_desc(sb + (F32 || alt ? 0 : t * C::BYTES), 16);
+          const uint32_t d = tm + CK_S + t * 128;
+          if (lead) {
+#pragma unroll
+            for (int part = 0; part < (F32 ? 2 : 1); ++part)  // fp32 rows: lo, then hi
+#pragma unroll
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t o = ((kk >> 2) * CK_TILE + (kk & 3) * 32) >> 4;
+                ck_mma_ss(d, qd + (F32 ? (1 - part) * C::BYTES >> 4 : 0) + o, kd + o, ID_S, (part | kk) != 0);
+              }
+            ck_commit(&s_full[t]);
+            if (alt || t == 1) ck_commit(&k_empty[st]);
+          }
+          __syncwarp();
+        }
+      }
+      fill += nt;
+    }
+    if (lead) ck_commit(&idle);  // completes once every MMA issued above is done
   } else {
     // ======== softmax: thread = row
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // row of its tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tm = tmem + lanes + CK_S + t * 128, o_tm = tmem + lanes + CK_O + t * 128;
-    unsigned fill = 0, ns = 0, no = 0, nw = 0;
+    unsigned fill = 0, ns = 0, no = 0;
     bool dead = false;
     auto pair_bar = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-    auto group_bar = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory"); };
-    // The group's first warp issues its MMAs: the warp walks together and one
-    // elected lane issues, so that descriptors stay in uniform registers (eight
-    // MMAs issue in 70 to 130 cycles where a lone thread took 390; they run
-    // for 515)
-    const bool issuer = (warp & 3) == 0, lead = issuer && ck_elect();
-    constexpr uint32_t ID_S = ck_idesc(128, false), ID_O = ck_idesc(HD, true);
-    const uint32_t sb32 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const int tt = __shfl_sync(0xffffffffu, t, 0);
     for (unsigned u = u0; u < u1;) {
       CkSeg x;
       const unsigned un = segment(u, x);
@@ -591,6 +655,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           if constexpr (F32) *reinterpret_cast<uint4*>(at + C::BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ck_arrive(&q_full);
       }
       const float slope = a.slopes && ok ? __ldg(a.slopes + head) * KVQ_LOG2E : 0.f;
       // keys that every row of the block sees; this row's own limits
@@ -600,234 +666,182 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       float m = -INFINITY, l = 0.f, ref = 0.f;
       int ev = -100;
       const int J = x.alt ? nt : 2 * nt;
-      ck_fence_before();
-      pair_bar();  // Q is in shared memory
-      // S of step j: this group's row tile, key tile j (alternating) or j / 2
-      auto ask_s = [&](int j) {
-        const unsigned f = fill + (x.alt ? j : j >> 1);
-        const int st = f & 1;
-        if (!wait(&k_full[st], f >> 1)) return false;
-        ck_fence_after();
-        if (lead) {
-          const uint64_t kd = ck_desc(sb32 + C::OFF_K + st * C::BYTES, 16);
-          const uint64_t qd = ck_desc(sb32 + (F32 || x.alt ? 0 : tt * C::BYTES), 16);
-          const uint32_t d = tm + CK_S + tt * 128;
-#pragma unroll
-          for (int part = 0; part < (F32 ? 2 : 1); ++part)  // fp32 rows: lo, then hi
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-              const uint32_t o = ((kk >> 2) * CK_TILE + (kk & 3) * 32) >> 4;
-              ck_mma_ss(d, qd + (F32 ? (1 - part) * C::BYTES >> 4 : 0) + o, kd + o, ID_S, (part | kk) != 0);
-            }
-          ck_commit(&s_full[tt]);
-          ck_commit(&k_empty[st]);
-          if (x.alt) ck_commit(&k_empty[st]);
-        }
-        __syncwarp();
-        return true;
-      };
-      // a warp that gave up keeps the group's barriers and skips the rest;
-      // step t - 2 only asks for the first S
 #pragma unroll 1
-      for (int j = t - 2; j < J; j += 2) {
+      for (int j = t; j < J && !dead; j += 2) {
         const int kt = x.alt ? j : j >> 1, j0 = x.key(x.lo + kt);
         const unsigned f = fill + kt;
         const int st = f & 1;
-        if (j >= 0 && !dead) dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns++);
-        if (j >= 0 && !dead) {
-          ck_fence_after();
-          const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
-          const float4* vsc = ksc + 32;
-          const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
-          // x of columns GC c .. GC c + GC - 1; where the common tile has its own
-          // code this one is kept small
-          constexpr int GC = PLAIN && !F32 ? 8 : 32;  // (fp32 rows' low parts go to columns that have to be read first)
-          auto scores = [&](int c, float (&z)[GC]) {
-            ck_get<GC>(s_tm + GC * c, z);
+        dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns++);
+        if (dead) break;
+        ck_fence_after();
+        const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
+        const float4* vsc = ksc + 32;
+        const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
+        // x of columns GC c .. GC c + GC - 1; where the common tile has its own
+        // code this one is kept small
+        constexpr int GC = PLAIN && !F32 ? 8 : 32;  // (fp32 rows' low parts go to columns that have to be read first)
+        auto scores = [&](int c, float (&z)[GC]) {
+          ck_get<GC>(s_tm + GC * c, z);
 #pragma unroll
-            for (int i = 0; i < GC / 4; ++i) {
-              const float4 k4 = ksc[GC / 4 * c + i];
-              const float k[4] = {k4.x, k4.y, k4.z, k4.w};
+          for (int i = 0; i < GC / 4; ++i) {
+            const float4 k4 = ksc[GC / 4 * c + i];
+            const float k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) z[4 * i + e] *= F32 ? k[e] * rmul : k[e];
-            }
-            if (!PLAIN && a.cap > 0.f) {
+            for (int e = 0; e < 4; ++e) z[4 * i + e] *= F32 ? k[e] * rmul : k[e];
+          }
+          if (!PLAIN && a.cap > 0.f) {
 #pragma unroll
-              for (int i = 0; i < GC; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
-            }
-            if (!PLAIN && a.slopes) {
+            for (int i = 0; i < GC; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
+          }
+          if (!PLAIN && a.slopes) {
 #pragma unroll
-              for (int i = 0; i < GC; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + GC * c + i))), z[i]);
-            }
-            if (!inner) {
+            for (int i = 0; i < GC; ++i) z[i] = fmaf(-slope, fabsf((float)(pos - (j0 + GC * c + i))), z[i]);
+          }
+          if (!inner) {
 #pragma unroll
-              for (int i = 0; i < GC; ++i) {
-                const int k = j0 + GC * c + i;
-                if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
-              }
-            }
-          };
-          // Does the reference hold? The common tile (no cap, no bias, nothing
-          // masked) asks a bound first, the largest raw product of 32 keys times
-          // their largest K scale, which needs no key's own scale.
-          const bool fast = PLAIN && inner;
-          const int en = max(ev, min(100, (int)(max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3])) >> 23) - 126));
-          float mx = m;
-          if (fast) {
-            float z[2][32];
-            ck_ld32(s_tm, z[0]);
-#pragma unroll 1
-            for (int c2 = 0; c2 < 4; c2 += 2)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = c2 + h;
-              ck_wait_ld(z[h]);
-              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
-              float(&w)[32] = z[h];
-              float top[2] = {0.f, 0.f};
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                top[0] = fmaxf(top[0], fmaxf(w[i], w[i + 1]));
-                top[1] = fmaxf(top[1], fmaxf(w[i + 2], w[i + 3]));
-              }
-              if (__any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) * (__uint_as_float(skm_s[st][c]) * rmul) <= m + CkLift<F32>::MARGIN))) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float4 k4 = ksc[8 * c + i];
-                  const float e0 = fmaxf(w[4 * i] * k4.x, w[4 * i + 1] * k4.y), e1 = fmaxf(w[4 * i + 2] * k4.z, w[4 * i + 3] * k4.w);
-                  mx = fmaxf(mx, fmaxf(e0, e1) * rmul);
-                }
-              }
-            }
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < 128 / GC; ++c) {
-              float z[GC];
-              scores(c, z);
-#pragma unroll
-              for (int i = 0; i < GC; ++i) mx = fmaxf(mx, z[i]);
+            for (int i = 0; i < GC; ++i) {
+              const int k = j0 + GC * c + i;
+              if (!((k >= r_lo && k <= r_hi) || k < x.pre)) z[i] = -INFINITY;
             }
           }
-          if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
-            const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT + (float)en;
-            const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
-            m = mx;
-            ev = en;
-            ref = rn;
-            l *= fac;
-            if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
+        };
+        // Does the reference hold? The common tile (no cap, no bias, nothing
+        // masked) asks a bound first, the largest raw product of 32 keys times
+        // their largest K scale, which needs no key's own scale.
+        const bool fast = PLAIN && inner;
+        const int en = max(ev, min(100, (int)(max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3])) >> 23) - 126));
+        float mx = m;
+        if (fast) {
+          float z[2][32];
+          ck_ld32(s_tm, z[0]);
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                float o[32];
-                ck_get32(o_tm + 32 * c, o);
+          for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= fac;
-                ck_st32(o_tm + 32 * c, o);
-              }
+          for (int h = 0; h < 2; ++h) {
+            const int c = c2 + h;
+            ck_wait_ld(z[h]);
+            if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
+            float(&w)[32] = z[h];
+            float top[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              top[0] = fmaxf(top[0], fmaxf(w[i], w[i + 1]));
+              top[1] = fmaxf(top[1], fmaxf(w[i + 2], w[i + 3]));
             }
-          }
-          if (fast) {
-            float z[2][32];
-            ck_ld32(s_tm, z[0]);
-            const float2 nref = make_float2(-ref, -ref);
-            float2 l2[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-            for (int c2 = 0; c2 < 4; c2 += 2)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = c2 + h;
-              ck_wait_ld(z[h]);
-              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
-              float(&w)[32] = z[h];
-              uint32_t ph[16], pl[F32 ? 16 : 1];
+            if (__any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) * (__uint_as_float(skm_s[st][c]) * rmul) <= m + CkLift<F32>::MARGIN))) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float4 k4 = ksc[8 * c + i], v4 = vsc[8 * c + i];
-                float2 u0 = make_float2(w[4 * i], w[4 * i + 1]), u1 = make_float2(w[4 * i + 2], w[4 * i + 3]);
-                if constexpr (F32) {
-                  u0 = mul2(u0, make_float2(rmul, rmul));
-                  u1 = mul2(u1, make_float2(rmul, rmul));
-                }
-                u0 = fma2(u0, make_float2(k4.x, k4.y), nref);
-                u1 = fma2(u1, make_float2(k4.z, k4.w), nref);
-                u0.x = ex2(u0.x); u0.y = ex2(u0.y); u1.x = ex2(u1.x); u1.y = ex2(u1.y);
-                l2[0] = add2(l2[0], u0);
-                l2[1] = add2(l2[1], u1);
-                u0 = mul2(u0, make_float2(v4.x, v4.y));
-                u1 = mul2(u1, make_float2(v4.z, v4.w));
-                if constexpr (F32) {
-                  ph[2 * i] = split_h2(u0.x, u0.y, pl[2 * i]);
-                  ph[2 * i + 1] = split_h2(u1.x, u1.y, pl[2 * i + 1]);
-                } else {
-                  ph[2 * i] = half2_bits(__floats2half2_rn(u0.x, u0.y));
-                  ph[2 * i + 1] = half2_bits(__floats2half2_rn(u1.x, u1.y));
-                }
+                const float4 k4 = ksc[8 * c + i];
+                const float e0 = fmaxf(w[4 * i] * k4.x, w[4 * i + 1] * k4.y), e1 = fmaxf(w[4 * i + 2] * k4.z, w[4 * i + 3] * k4.w);
+                mx = fmaxf(mx, fmaxf(e0, e1) * rmul);
               }
-              ck_st16(s_tm + 32 * c, ph);
-              if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
             }
-            l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-          } else {
+          }
+        } else {
 #pragma unroll 1
-            for (int c = 0; c < 128 / GC; ++c) {
-              float z[GC];
-              scores(c, z);
-              uint32_t ph[GC / 2], pl[F32 ? GC / 2 : 1];
+          for (int c = 0; c < 128 / GC; ++c) {
+            float z[GC];
+            scores(c, z);
 #pragma unroll
-              for (int i = 0; i < GC / 4; ++i) {
-                const float4 v4 = vsc[GC / 4 * c + i];
-                const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
-                float p[4];
+            for (int i = 0; i < GC; ++i) mx = fmaxf(mx, z[i]);
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
+          const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT + (float)en;
+          const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
+          m = mx;
+          ev = en;
+          ref = rn;
+          l *= fac;
+          if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              float o[32];
+              ck_get32(o_tm + 32 * c, o);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float y = ex2(z[4 * i + e] - ref);
-                  l += y;
-                  p[e] = y == 0.f ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
-                }
-                if constexpr (F32) {
-                  ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
-                  ph[2 * i + 1] = split_h2(p[2], p[3], pl[2 * i + 1]);
-                } else {
-                  ph[2 * i] = half2_bits(__floats2half2_rn(p[0], p[1]));
-                  ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
-                }
-              }
-              // keys 32 k ..: 16 columns of pairs at 32 k (and 16 of low parts).
-              // GC = 8 overwrites columns 32 k + 4 r ..: of chunk r = 0 the first
-              // four of its own, later ones columns that were read before.
-              const uint32_t to = s_tm + (GC * c & ~31) + (GC * c & 31) / 2;
-              ck_put<GC / 2>(to, ph);
-              if constexpr (F32) ck_put<GC / 2>(to + 16, pl);
+              for (int i = 0; i < 32; ++i) o[i] *= fac;
+              ck_st32(o_tm + 32 * c, o);
             }
           }
-          ck_wait_st();
-          ck_fence_before();
         }
-        if (j >= 0) group_bar();  // the group's P (and rescaled O) is complete
-        // The groups issue in turn, P V and the next S together: their tiles
-        // then run on the tensor pipe one after the other, and one group
-        // exponentiates while the other's run (left alone both fall into step).
-        if (issuer && !dead) {
-          if (j > 0) dead = !wait(&turn[t], nw++);
-          ck_fence_after();
-          if (lead && !dead && j >= 0) {
-            const uint64_t vd = ck_desc(sb32 + C::OFF_V + st * C::BYTES, CK_TILE);
-            const uint32_t d = tm + CK_O + tt * 128, p = tm + CK_S + tt * 128;
-            const int fresh = j < 2;  // this group's first tile: O starts here
+        if (fast) {
+          float z[2][32];
+          ck_ld32(s_tm, z[0]);
+          const float2 nref = make_float2(-ref, -ref);
+          float2 l2[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+          for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
-            for (int part = 0; part < (F32 ? 2 : 1); ++part)
+          for (int h = 0; h < 2; ++h) {
+            const int c = c2 + h;
+            ck_wait_ld(z[h]);
+            if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
+            float(&w)[32] = z[h];
+            uint32_t ph[16], pl[F32 ? 16 : 1];
 #pragma unroll
-              for (int kk = 0; kk < CK_KEYS / 16; ++kk)
-                ck_mma_ts(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + (F32 ? (1 - part) * 16 : 0), vd + kk * (2048 >> 4), ID_O,
-                          (part | kk) != 0 || !fresh);
-            ck_commit(&v_empty[st]);
-            if (x.alt) ck_commit(&v_empty[st]);
-            if (j + 2 >= J) ck_commit(&o_full[tt]);
+            for (int i = 0; i < 8; ++i) {
+              const float4 k4 = ksc[8 * c + i], v4 = vsc[8 * c + i];
+              float2 u0 = make_float2(w[4 * i], w[4 * i + 1]), u1 = make_float2(w[4 * i + 2], w[4 * i + 3]);
+              if constexpr (F32) {
+                u0 = mul2(u0, make_float2(rmul, rmul));
+                u1 = mul2(u1, make_float2(rmul, rmul));
+              }
+              u0 = fma2(u0, make_float2(k4.x, k4.y), nref);
+              u1 = fma2(u1, make_float2(k4.z, k4.w), nref);
+              u0.x = ex2(u0.x); u0.y = ex2(u0.y); u1.x = ex2(u1.x); u1.y = ex2(u1.y);
+              l2[0] = add2(l2[0], u0);
+              l2[1] = add2(l2[1], u1);
+              u0 = mul2(u0, make_float2(v4.x, v4.y));
+              u1 = mul2(u1, make_float2(v4.z, v4.w));
+              if constexpr (F32) {
+                ph[2 * i] = split_h2(u0.x, u0.y, pl[2 * i]);
+                ph[2 * i + 1] = split_h2(u1.x, u1.y, pl[2 * i + 1]);
+              } else {
+                ph[2 * i] = half2_bits(__floats2half2_rn(u0.x, u0.y));
+                ph[2 * i + 1] = half2_bits(__floats2half2_rn(u1.x, u1.y));
+              }
+            }
+            ck_st16(s_tm + 32 * c, ph);
+            if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
           }
-          __syncwarp();
-          if (!dead && j + 2 < J) dead = !ask_s(j + 2);
-          if (lane == 0 && j >= 0 && j + 1 < J) ck_arrive(&turn[t ^ 1]);
+          l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 128 / GC; ++c) {
+            float z[GC];
+            scores(c, z);
+            uint32_t ph[GC / 2], pl[F32 ? GC / 2 : 1];
+#pragma unroll
+            for (int i = 0; i < GC / 4; ++i) {
+              const float4 v4 = vsc[GC / 4 * c + i];
+              const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+              float p[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y = ex2(z[4 * i + e] - ref);
+                l += y;
+                p[e] = y == 0.f ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
+              }
+              if constexpr (F32) {
+                ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
+                ph[2 * i + 1] = split_h2(p[2], p[3], pl[2 * i + 1]);
+              } else {
+                ph[2 * i] = half2_bits(__floats2half2_rn(p[0], p[1]));
+                ph[2 * i + 1] = half2_bits(__floats2half2_rn(p[2], p[3]));
+              }
+            }
+            // keys 32 k ..: 16 columns of pairs at 32 k (and 16 of low parts).
+            // GC = 8 overwrites columns 32 k + 4 r ..: of chunk r = 0 the first
+            // four of its own, later ones columns that were read before.
+            const uint32_t to = s_tm + (GC * c & ~31) + (GC * c & 31) / 2;
+            ck_put<GC / 2>(to, ph);
+            if constexpr (F32) ck_put<GC / 2>(to + 16, pl);
+          }
         }
+        ck_wait_st();
+        ck_fence_before();
+        __syncwarp();
+        if (lane == 0) ck_arrive(&p_full[t]);
       }
       fill += nt;
 
@@ -976,11 +990,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       }
       u = un;
     }
-    if (lead) ck_commit(&idle);  // completes once every MMA this lane issued is done
   }
   ck_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == CK_MMA) {
     if (lane == 0) mbar_wait_bounded(&idle, 0u, MBAR_SPIN_LIMIT);  // no MMA may still write the memory that is freed
     __syncwarp();
     ck_fence_after();
