@@ -2,10 +2,18 @@
 // the choice between the two kernels.
 //
 // A sequence of few packed rows (new rows x query heads per KV head) is bound
-// by its cache's bytes and goes to the decode kernel (kvq_decode.cu); one of
-// many rows by the tensor pipe and goes to the chunk kernel (kvq_chunk.cu).
-// Each kernel takes its own sequences out of the batch, so a batch may mix
-// them.
+// by its cache's bytes and goes to the decode kernel (kvq_decode.cu), in up to
+// four tasks of 16 rows per KV head; one of more rows is bound by the tensor
+// pipe and goes to the chunk kernel (kvq_chunk.cu). Each kernel takes its own
+// sequences out of the batch, so a batch may mix them. Decode / chunk kernel,
+// int8, head dim 128, 8 KV heads, lengths up to 4096:
+//   8 sequences,  20 packed rows    37 /  58 us
+//   8 sequences,  64 packed rows    58 /  66 us
+//   8 sequences, 128 packed rows    96 /  80 us
+//   32 sequences, 32 packed rows    95 / 136 us
+//   32 sequences, 64 packed rows   172 / 146 us
+// Beside a sequence for the chunk kernel the others mostly bring one row, so
+// the decode kernel's blocks are 8 rows there.
 #include <cmath>
 
 #include "kvq_attend.cuh"
@@ -18,10 +26,12 @@ template <int HD, int BITS, typename T>
 int attend_launch(AttendArgs a, cudaStream_t s) {
   // a batch of equal row counts needs one of the two kernels only
   const long long max_packed = (long long)a.v.max_rows * a.G;
-  a.few = max_packed <= KVQ_DECODE_ROWS ? KVQ_DECODE_ROWS : a.G <= 8 ? 8 : KVQ_DECODE_ROWS;
   const bool equal = (long long)a.v.max_rows * a.v.n_seq == a.v.n_rows;
-  if (max_packed <= a.few || !equal) {
-    const int rc = kvq_decode_launch<HD, BITS, T>(a, (int)min(max_packed, (long long)a.few), s);
+  const int most = KVQ_DECODE_BLOCKS * KVQ_DECODE_ROWS;
+  const int rows = max_packed <= 8 || (max_packed > most && a.G <= 8) ? 8 : KVQ_DECODE_ROWS;  // of a decode block
+  a.few = a.G <= rows ? KVQ_DECODE_BLOCKS * rows : 0;
+  if (a.few && (max_packed <= a.few || !equal)) {
+    const int rc = kvq_decode_launch<HD, BITS, T>(a, rows, s);
     if (rc) return rc;
   }
   return max_packed <= a.few ? LUMINA_OK : kvq_chunk_launch<HD, BITS, T>(a, s);

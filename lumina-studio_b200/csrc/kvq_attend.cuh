@@ -9,7 +9,8 @@ namespace lumina {
 
 constexpr int KVQ_MAX_CTAS = 512;    // CTAs that may leave partial states (two each)
 constexpr int KVQ_FAN = 64;          // partial states that one CTA joins at a time
-constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of one sequence the decode kernel takes at most
+constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of a decode task at most
+constexpr int KVQ_DECODE_BLOCKS = 4;  // tasks of one sequence and KV head at most
 
 struct AttendArgs {
   KvqView v;
@@ -28,9 +29,9 @@ struct AttendArgs {
   long long spin;
 };
 
-// sequences of up to a.few packed rows, at most max_packed of them (kvq_decode.cu)
+// sequences of up to a.few packed rows, in blocks of up to `rows` (8 or 16; kvq_decode.cu)
 template <int HD, int BITS, typename T>
-int kvq_decode_launch(AttendArgs a, int max_packed, cudaStream_t s);
+int kvq_decode_launch(AttendArgs a, int rows, cudaStream_t s);
 
 // sequences of more than a.few packed rows (kvq_chunk.cu)
 template <int HD, int BITS, typename T>

@@ -1,8 +1,10 @@
 // Attention of sequences with few new rows (decode steps, short drafts) over
 // quantized KV pages: bound by the bytes of the cache.
 //
-// A task is one (KV head, sequence): up to 8 NR packed query rows (row r =
-// local row r / G, head r % G). Its keys are cut into cells of 32. All cells
+// A task is one (KV head, sequence, block of its new rows): up to 8 NR packed
+// query rows (row r = local row r / G, head r % G); the blocks of one
+// sequence share its keys through the L2. A task's keys are cut into cells of
+// 32 (16 where the registers hold no more). All cells
 // of all tasks form one line that the CTAs share evenly, so lengths may be as
 // ragged as they like; a task that spans CTAs leaves partial states in the
 // workspace, which the CTAs that arrive last join in part order (the result
@@ -50,10 +52,11 @@ struct DecCfg {
   static constexpr int SMEM = W * SLAB > JOIN ? W * SLAB : JOIN;  // + n_seq ints
 };
 
-// One segment: cells [lo, hi) of the cell line of (KV head, sequence).
+// One segment: cells [lo, hi) of the cell line of a task.
 struct Seg {
-  int s, kvh, lo, hi, total;  // total: the task's cells
-  int first, n, len, pre, tp, tl;
+  int s, kvh, lo, hi, total, blocks;  // total: the task's cells; blocks: the sequence's tasks of one KV head
+  int first, n, len, pre, tp, tl;     // n rows from batch row `first`
+  int p0;                             // position of the first
   __device__ __forceinline__ int at(int c) const { return c < tp ? c : c - tp + tl; }  // cell c's place in the cache, in cells
 };
 
@@ -81,6 +84,7 @@ kvq_decode_kernel(AttendArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const KvqView& v = a.v;
   const int cap_tokens = v.pages_ld << v.page_shift;
+  const int block_rows = R / a.G;  // the launch has G <= R
 
   // what the batch says about sequence s (0 rows: not this kernel's)
   auto describe = [&](int s, Seg& x, bool report) {
@@ -98,6 +102,8 @@ kvq_decode_kernel(AttendArgs a) {
     x.tp = (x.pre + CELL - 1) / CELL;
     x.tl = max(x.tp, lo / CELL);
     x.total = x.n ? max(1, x.tp + max(x.tl, (x.len + CELL - 1) / CELL) - x.tl) : 0;
+    x.blocks = (x.n + block_rows - 1) / block_rows;
+    x.p0 = p_lo;
   };
 
   // the cell line
@@ -105,9 +111,9 @@ kvq_decode_kernel(AttendArgs a) {
   for (int s0 = 0; s0 < v.n_seq; s0 += C::THREADS) {
     const int s = s0 + tid;
     Seg x;
-    x.total = 0;
+    x.total = x.blocks = 0;
     if (s < v.n_seq) describe(s, x, blockIdx.x == 0);
-    int inc = x.total;
+    int inc = x.total * x.blocks;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const int y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -144,7 +150,11 @@ kvq_decode_kernel(AttendArgs a) {
     describe(lo, x, false);
     x.kvh = kvh;
     const int base = lo ? cells[lo - 1] : 0;
-    x.lo = c - base;
+    const int b = (c - base) / x.total;
+    x.lo = c - base - b * x.total;
+    x.first += b * block_rows;
+    x.p0 += b * block_rows;
+    x.n = min(block_rows, x.n - b * block_rows);
     x.hi = min(x.total, x.lo + (int)(u1 - u));
   };
 
@@ -331,7 +341,7 @@ kvq_decode_kernel(AttendArgs a) {
         qmul[o][c] = __shfl_sync(0xffffffffu, mul, (2 * t + c) * 4);
         if constexpr (OFFSET) off[o][c] = __shfl_sync(0xffffffffu, of, (2 * t + c) * 4);
         const int li = rr < x.n * a.G ? rr / a.G : 0;
-        pos[o][c] = x.len - x.n + li;
+        pos[o][c] = x.p0 + li;
         if constexpr (!PLAIN)
           slope[o][c] = a.slopes && rr < x.n * a.G ? __ldg(a.slopes + x.kvh * a.G + rr - li * a.G) * KVQ_LOG2E : 0.f;
       }
@@ -355,8 +365,8 @@ kvq_decode_kernel(AttendArgs a) {
 
     // cells that start in [in_lo, in_hi] are seen by every row, as are those
     // that end within the prefix
-    const int in_lo = a.window ? x.len - a.window : 0, in_hi = min(x.len - x.n + 1, x.len) - CELL, in_pre = x.pre - CELL;
-    const int win_any = a.window ? x.len - x.n - a.window + 1 : -0x7fffffff;  // keys from here: some row
+    const int in_lo = a.window ? x.p0 + x.n - a.window : 0, in_hi = min(x.p0 + 1, x.len) - CELL, in_pre = x.pre - CELL;
+    const int win_any = a.window ? x.p0 - a.window + 1 : -0x7fffffff;  // keys from here: some row
     for (int c = x.lo + warp; c < x.hi; c += W) {
       const int j0 = jn;
       const unsigned held = have;
@@ -751,8 +761,8 @@ int decode_nr(const AttendArgs& a, cudaStream_t s) {
 }  // namespace
 
 template <int HD, int BITS, typename T>
-int kvq_decode_launch(AttendArgs a, int max_packed, cudaStream_t s) {
-  return max_packed <= 8 ? decode_nr<HD, BITS, 1, T>(a, s) : decode_nr<HD, BITS, 2, T>(a, s);
+int kvq_decode_launch(AttendArgs a, int rows, cudaStream_t s) {
+  return rows == 8 ? decode_nr<HD, BITS, 1, T>(a, s) : decode_nr<HD, BITS, 2, T>(a, s);
 }
 template int kvq_decode_launch<128, 8, __half>(AttendArgs, int, cudaStream_t);
 template int kvq_decode_launch<128, 8, float>(AttendArgs, int, cudaStream_t);

@@ -292,6 +292,23 @@ def test_attend_rows_that_see_nothing(sv, io):
     check_attend(got, want, io)
 
 
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("heads,n_kv,rows,lens,cap,alibi,window,prefix", [
+    (8, 2, [5, 5, 5], [700, 5, 33], 0.0, False, 0, None),          # 20 packed rows: one and a quarter blocks of 16
+    (16, 1, [4, 1, 0, 3], [129, 64, 50, 3], 20.0, False, 0, None),  # a row a block
+    (12, 1, [5, 2], [400, 2], 0.0, True, 0, None),                  # blocks of one row of 12 heads
+    (6, 2, [21, 7, 20], [300, 7, 4100], 0.0, False, 150, [0, 7, 40]),  # 63 packed rows, blocks of 5 rows of 3 heads
+    (3, 3, [64, 16, 17], [64, 1500, 17], 30.0, True, 40, [9, 0, 17]),  # one head each: four blocks
+    (14, 2, [90, 4, 1, 3], [700, 444, 2000, 3], 0.0, False, 100, [20, 0, 5, 0]),  # beside a chunk: blocks of 8
+])
+def test_attend_row_blocks(sv, io, heads, n_kv, rows, lens, cap, alibi, window, prefix):
+    """Sequences whose rows are split over several tasks of one KV head."""
+    got, want = run_attend(sv, 8, 64, io, heads, n_kv, 32, rows, lens, cap, alibi, window, prefix, seed=7)
+    assert rel(got, want) < TOL[io]
+    got, want = run_attend(sv, 4, 128, io, heads, n_kv, 16, rows, lens, cap, alibi, window, prefix, seed=8)
+    assert rel(got, want) < TOL[io]
+
+
 @pytest.mark.parametrize("rows", [1, 50])
 def test_attend_long(sv, rows):
     got, want = run_attend(sv, 4, 64, "float32", 4, 1, 128, [rows], [20011], seed=11)
