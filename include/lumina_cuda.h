@@ -342,7 +342,9 @@ typedef struct {
  * row_start[n_seq]; max_rows is at least every sequence's row count; a
  * sequence may have no rows. The kernels check these device values: a row,
  * length or page number out of range sets bit 64 of the device fault word
- * (lumina_fault_status) and the affected rows are skipped. */
+ * (lumina_fault_status); append and read skip the rows it concerns, attend
+ * leaves the rows of that sequence unspecified and serves the others. Pages
+ * that no token below len lies on may hold any number. */
 typedef struct {
   const int* row_start_dev; /* n_seq + 1 */
   const int* len_dev;       /* n_seq */
@@ -386,7 +388,11 @@ int lumina_kvq_read(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch, 
  * `type`; scores, softmax statistics and sums are fp32. workspace_dev: at
  * least lumina_kvq_workspace_bytes, zeroed once by the caller before its
  * first use and left reusable by every call; calls that may overlap on the
- * GPU need workspaces of their own. */
+ * GPU need workspaces of their own. The order of every sum is fixed by the
+ * batch's lengths, so equal calls give equal bits. The sequences' lengths
+ * times n_kv add up to less than 2^31 (bit 64 and no output otherwise). A wait inside
+ * that gives up sets bit 32 and leaves outputs unwritten. At most 128 query
+ * heads per KV head. */
 typedef struct {
   const void* q_dev;
   void* out_dev;
@@ -405,8 +411,8 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
                       void* stream);
 int lumina_kvq_workspace_bytes(int device, size_t* bytes);
 
-/* Shape logits rows (rows x vocab float32, ld elements apart) into out (may
- * be the input): for every token t that occurs c > 0 times in the row's
+/* Shape logits rows (rows x vocab float32, ld elements apart) into out (the
+ * input itself or a buffer apart from it): for every token t that occurs c > 0 times in the row's
  * history, l = l > 0 ? l / repeat : l * repeat (the sampler's rule,
  * chat.py:330-338), then l = l - frequency * c - presence; then l += bias of
  * the row's (token, value) list (a token listed twice takes its last entry);
@@ -421,12 +427,14 @@ typedef struct {
   int rows, vocab;
   const int* hist_start_dev;  /* rows + 1 offsets into hist_tok, or NULL */
   const int* hist_tok_dev;
+  int hist_len;               /* tokens in hist_tok: offsets are kept within 0..hist_len */
   const float* repeat_dev;    /* rows, > 0, or NULL (1) */
   const float* frequency_dev; /* rows, or NULL (0) */
   const float* presence_dev;  /* rows, or NULL (0) */
   const int* bias_start_dev;  /* rows + 1 offsets, or NULL */
   const int* bias_tok_dev;
   const float* bias_val_dev;
+  int bias_len;               /* entries in bias_tok and bias_val, likewise */
   const uint32_t* mask_dev;   /* rows x mask_ld words, or NULL */
   int mask_ld;
   int* argmax_dev;            /* rows, or NULL */

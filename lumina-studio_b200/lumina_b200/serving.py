@@ -50,9 +50,10 @@ class _Attend(ctypes.Structure):
 
 class _Logits(ctypes.Structure):
     _fields_ = [("logits_dev", _VP), ("out_dev", _VP), ("ld", _I), ("ldo", _I), ("rows", _I), ("vocab", _I),
-                ("hist_start_dev", _VP), ("hist_tok_dev", _VP), ("repeat_dev", _VP), ("frequency_dev", _VP),
-                ("presence_dev", _VP), ("bias_start_dev", _VP), ("bias_tok_dev", _VP), ("bias_val_dev", _VP),
-                ("mask_dev", _VP), ("mask_ld", _I), ("argmax_dev", _VP), ("device", _I)]
+                ("hist_start_dev", _VP), ("hist_tok_dev", _VP), ("hist_len", _I), ("repeat_dev", _VP),
+                ("frequency_dev", _VP), ("presence_dev", _VP), ("bias_start_dev", _VP), ("bias_tok_dev", _VP),
+                ("bias_val_dev", _VP), ("bias_len", _I), ("mask_dev", _VP), ("mask_ld", _I), ("argmax_dev", _VP),
+                ("device", _I)]
 
 
 def _bad(text: str):
@@ -268,6 +269,7 @@ def adjust_logits(logits, history=None, repeat=None, frequency=None, presence=No
     if history is not None and history[1].numel():
         a.hist_start_dev = _vec(history[0], torch.int32, dev, "history offsets", R + 1)
         a.hist_tok_dev = _vec(history[1], torch.int32, dev, "history tokens")
+        a.hist_len = history[1].numel()
     if repeat is not None:
         a.repeat_dev = _vec(repeat, torch.float32, dev, "repeat", R)
     if frequency is not None:
@@ -278,6 +280,7 @@ def adjust_logits(logits, history=None, repeat=None, frequency=None, presence=No
         a.bias_start_dev = _vec(bias[0], torch.int32, dev, "bias offsets", R + 1)
         a.bias_tok_dev = _vec(bias[1], torch.int32, dev, "bias tokens")
         a.bias_val_dev = _vec(bias[2], torch.float32, dev, "bias values", bias[1].numel())
+        a.bias_len = bias[1].numel()
     if mask is not None:
         a.mask_dev = _vec(mask, torch.int32, dev, "mask")
         a.mask_ld = mask.shape[1]

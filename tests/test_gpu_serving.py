@@ -473,6 +473,71 @@ def test_out_of_range_data_is_reported(sv):
     assert cuda.fault_status(0) == sv.FAULT_DATA
 
 
+@pytest.mark.parametrize("io", ["float16", "float32"])
+def test_attend_wait_that_gives_up(sv, io):
+    """The chunk kernel's waits given no polls at all: fault bit 32 and a
+    return; the next call is right (nothing of the failed one is left in the
+    workspace)."""
+    import torch
+    from lumina_b200 import cuda
+    rng = np.random.default_rng(14)
+    hd, page, heads, n_kv, rows, ln = 128, 16, 8, 2, 300, 2000
+    table, n_pages, _ = layout(rng, [ln], page)
+    pool = sv.KVPool(dev(random_pool(rng, n_pages, n_kv, 8, hd, page)), 8, hd, page)
+    q = dev(rng.standard_normal((rows, heads * hd)).astype(np.float32), getattr(torch, io))
+    batch = batch_of(sv, [rows], [ln], table)
+    good = pool.attend(batch, q).clone()
+    assert cuda.fault_status(0) == 0
+    cuda.debug_wait_limit(0)
+    try:
+        pool.attend(batch, q)
+        torch.cuda.synchronize()
+        assert cuda.fault_status(0) & sv.FAULT_WAIT
+    finally:
+        cuda.debug_wait_limit(-1)
+        cuda.fault_status(0, clear=True)
+    assert torch.equal(pool.attend(batch, q), good)
+    assert cuda.fault_status(0) == 0
+
+
+def test_attend_many_sequences(sv):
+    """More row blocks than the chunk kernel lines up one by one, some of
+    them without rows or tokens."""
+    rng = np.random.default_rng(15)
+    lens = rng.integers(0, 40, 2100).tolist()
+    rows = [int(rng.integers(0, 2)) if i % 7 == 0 else 1 for i in range(2100)]
+    got, want = run_attend(sv, 8, 64, "float32", 72, 1, 16, rows, lens, seed=16)
+    check_attend(got, want, "float32")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_pages_past_4_gib(sv, rows):
+    """The pages of a sequence at both ends of a pool of 5 GiB."""
+    import torch
+    rng = np.random.default_rng(17)
+    hd, page, n_kv, heads, ln = 128, 16, 32, 64, 200
+    n_pages = (5 << 30) // (n_kv * ref.block_bytes(8, hd, page))
+    pool = sv.KVPool.empty(n_pages, n_kv, hd, 8, page)
+    need = -(-ln // page)
+    table = np.array([[n_pages - 1 - i if i % 2 else i for i in range(need)]], np.int32)
+    some = random_pool(rng, need, n_kv, 8, hd, page)
+    pool.data[torch.from_numpy(table[0].astype(np.int64)).cuda()] = dev(some)
+    q, k, v = (rng.standard_normal((rows, h * hd)).astype(np.float32) for h in (heads, n_kv, n_kv))
+    cs = dev(np.ones((ln, hd // 2), np.float32))
+    batch = batch_of(sv, [rows], [ln], table)
+    qr = pool.append(batch, dev(q), dev(k), dev(v), cs, dev(np.zeros((ln, hd // 2), np.float32)))
+    assert np.array_equal(qr.cpu().numpy().reshape(rows, -1), q)  # a rotation by nothing
+    got = pool.attend(batch, qr).cpu().numpy()
+    back = [x.cpu().numpy() for x in pool.read(batch)]
+    now = pool.data[torch.from_numpy(table[0].astype(np.int64)).cuda()].cpu().numpy()
+    kk, vv = ref.rows_of(now, np.arange(need, dtype=np.int32), ln, 8, hd, page)
+    for x, y, z in zip(back, (k, v), (kk, vv)):
+        y = y.reshape(rows, n_kv, hd)
+        assert np.abs(x - y).max() <= 0.5001 / 127 * np.abs(y).max()
+        assert rel(x, z[-rows:]) < 1e-6
+    assert rel(got, ref.attend(q.astype(np.float64).reshape(rows, heads, hd), kk, vv, ln, hd ** -0.5)) < TOL["float32"]
+
+
 def test_refusals(sv):
     import torch
     from lumina_b200.cuda import LuminaError
@@ -539,6 +604,8 @@ def test_no_rows(sv):
     (5, 1000, 17, 3, False, 3),
     (2, 131075, 300, 300, True, 1),
     (70, 257, 30, 0, True, 0),
+    (2, 131075, 20000, 40, True, 1),  # more named tokens than are counted at once
+    (1, 1200007, 9000, 50, True, 1),  # a CTA's part longer than the bits of named tokens
 ])
 def test_logits(sv, rows, vocab, hist, biases, masked, pad):
     import torch
