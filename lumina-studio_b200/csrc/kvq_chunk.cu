@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
         int c0 = 0, c1 = CH;
         if constexpr (F32) {
           uint32_t top = 0;
-#pragma unroll 4
+#pragma unroll 8
           for (int c = 0; c < HD / 4; ++c) {
             const float4 f = __ldg(reinterpret_cast<const float4*>(src) + c);
             top = max(max(top, __float_as_uint(f.x) & 0x7fffffffu), __float_as_uint(f.y) & 0x7fffffffu);
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           c1 = c0 + CH / 2;
         }
         const float up = F32 ? __int_as_float((254 << 23) - __float_as_int(rmul)) : 1.f;  // 1 / rmul
-#pragma unroll 2
+#pragma unroll 4
         for (int c = c0; c < c1; ++c) {
           float q[8];
           if constexpr (F32) {
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           }
           if (!PLAIN && a.cap > 0.f) {
 #pragma unroll
-            for (int i = 0; i < GC; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanhf(z[i]) : tanh_fast(z[i]));
+            for (int i = 0; i < GC; ++i) z[i] = a.cap * KVQ_LOG2E * (F32 ? tanh_f32(z[i]) : tanh_fast(z[i]));
           }
           if (!PLAIN && a.slopes) {
 #pragma unroll
@@ -744,7 +744,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             scores(c, z);
 #pragma unroll
             for (int i = 0; i < GC; ++i) mx = fmaxf(mx, z[i]);
+            if constexpr (GC == 32) ck_st32(s_tm + GC * c, z);  // tanh, bias and mask once only
           }
+          if constexpr (GC == 32) ck_wait_st();
         }
         if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
           const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT + (float)en;
@@ -809,7 +811,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
 #pragma unroll 1
           for (int c = 0; c < 128 / GC; ++c) {
             float z[GC];
-            scores(c, z);
+            if constexpr (GC == 32) ck_get32(s_tm + GC * c, z);
+            else scores(c, z);
             uint32_t ph[GC / 2], pl[F32 ? GC / 2 : 1];
 #pragma unroll
             for (int i = 0; i < GC / 4; ++i) {
@@ -933,7 +936,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             if (split) {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                __stcg(reinterpret_cast<float4*>(my_part + (size_t)(pr - x.row0) * HD + 32 * c) + i,
+                __stcg(reinterpret_cast<float4*>(my_part) + (8 * c + i) * BM + pr - x.row0,
                        make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
             } else {
               put(pr, c, o, inv);
@@ -955,34 +958,66 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
         }
         pair_bar();
         if (last_s) {
-          // thread: 4 dims of a row, the parts in order
+          // Rows' largest reference and sums first (the Q tiles are free),
+          // then 4 dims of four rows per thread and pass, the parts in order;
+          // eight lanes hold neighbouring rows, four neighbouring dims.
           const int np = ce - cb + 1;
-          for (int i = tid; i < x.rows * (HD / 4); i += 256) {
-            const int r = i / (HD / 4), d4 = i % (HD / 4);
+          float2* stat = reinterpret_cast<float2*>(sm);
+          auto stat_of = [&](int p) { return reinterpret_cast<const float2*>(a.ws + slot_of(p) * part + (size_t)BM * HD); };
+          if (tid < x.rows) {
             float M = -INFINITY, L = 0.f;
-            for (int p = 0; p < np; ++p)
-              M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(a.ws + slot_of(p) * part + (size_t)BM * HD) + r).x);
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
+            for (int p = 0; p < np; ++p) M = fmaxf(M, __ldcg(stat_of(p) + tid).x);
+#pragma unroll 8
             for (int p = 0; p < np; ++p) {
-              const float* at_p = a.ws + slot_of(p) * part;
-              const float2 rl = __ldcg(reinterpret_cast<const float2*>(at_p + (size_t)BM * HD) + r);
-              const float4 z = __ldcg(reinterpret_cast<const float4*>(at_p + (size_t)r * HD) + d4);
-              const float w = rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M);
-              L += rl.y * w;
-              y.x = fmaf(z.x, w, y.x); y.y = fmaf(z.y, w, y.y); y.z = fmaf(z.z, w, y.z); y.w = fmaf(z.w, w, y.w);
+              const float2 rl = __ldcg(stat_of(p) + tid);
+              L += rl.y * (rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M));
             }
-            const float inv = 1.0f / L;
-            if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
-            else y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-            const int packed = x.row0 + r, li2 = packed / a.G;
-            T* dst = static_cast<T*>(a.out) + (size_t)(x.first + li2) * a.ldo + (size_t)(x.kvh * a.G + packed - li2 * a.G) * HD;
-            if constexpr (BITS == 4) {
-              // columns 4 d4 .. + 3 hold dims b + {0, 4, 1, 5} or b + {2, 6, 3, 7}
-              const int b = (d4 >> 1) * 8 + 2 * (d4 & 1);
-              dst[b] = (T)y.x; dst[b + 4] = (T)y.y; dst[b + 1] = (T)y.z; dst[b + 5] = (T)y.w;
-            } else {
-              kvq_store4(dst + 4 * d4, y.x, y.y, y.z, y.w);
+            stat[tid] = make_float2(M, L);
+          }
+          pair_bar();
+          constexpr int K = 4;
+          const int octets = (x.rows + 7) / 8;  // items: (octet, four dims' quad, lane)
+          for (int i0 = tid; i0 < octets * (HD / 16) * 32; i0 += 256 * K) {
+            int r[K], d4[K];
+            float4 y[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              const int i = (i0 + 256 * k) >> 5, q = i / octets;
+              r[k] = (i - q * octets) * 8 + (lane & 7);
+              d4[k] = 4 * q + (lane >> 3);
+              if (q >= HD / 16 || r[k] >= x.rows) r[k] = -1;
+              y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll 2
+            for (int p = 0; p < np; ++p) {
+              const float4* at_p = reinterpret_cast<const float4*>(a.ws + slot_of(p) * part);
+#pragma unroll
+              for (int k = 0; k < K; ++k) {
+                if (r[k] < 0) continue;
+                const float2 rl = __ldcg(stat_of(p) + r[k]);
+                const float4 z = __ldcg(at_p + d4[k] * BM + r[k]);
+                const float w = rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - stat[r[k]].x);
+                y[k].x = fmaf(z.x, w, y[k].x); y[k].y = fmaf(z.y, w, y[k].y);
+                y[k].z = fmaf(z.z, w, y[k].z); y[k].w = fmaf(z.w, w, y[k].w);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              if (r[k] < 0) continue;
+              const float L = stat[r[k]].y, inv = 1.0f / L;
+              float4 o = y[k];
+              if (L == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+              else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+              const int packed = x.row0 + r[k], li2 = packed / a.G;
+              T* dst = static_cast<T*>(a.out) + (size_t)(x.first + li2) * a.ldo + (size_t)(x.kvh * a.G + packed - li2 * a.G) * HD;
+              if constexpr (BITS == 4) {
+                // columns 4 d4 .. + 3 hold dims b + {0, 4, 1, 5} or b + {2, 6, 3, 7}
+                const int b = (d4[k] >> 1) * 8 + 2 * (d4[k] & 1);
+                dst[b] = (T)o.x; dst[b + 4] = (T)o.y; dst[b + 1] = (T)o.z; dst[b + 5] = (T)o.w;
+              } else {
+                kvq_store4(dst + 4 * d4[k], o.x, o.y, o.z, o.w);
+              }
             }
           }
         }

@@ -448,7 +448,7 @@ kvq_decode_kernel(AttendArgs a) {
             for (int r = 0; r < NR; ++r)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                p[n][r][e] = a.cap * KVQ_LOG2E * (F32 ? tanhf(p[n][r][e]) : tanh_fast(p[n][r][e]));
+                p[n][r][e] = a.cap * KVQ_LOG2E * (F32 ? tanh_f32(p[n][r][e]) : tanh_fast(p[n][r][e]));
         }
 #pragma unroll
         for (int n = 0; n < NK; ++n)

@@ -11,7 +11,7 @@
 // Fragment layouts (lane = 4 g + t): in the K fragment of key g, a thread's
 // four k-indices of a step are any four dims as long as q uses the same, so
 // thread t owns runs of the key's codes that load as 16-byte words
-// (dim_of). In the V fragment, n-tile i takes dim g * HD / 8 + i at column
+// (load_q takes q's dims in that order). In the V fragment, n-tile i takes dim g * HD / 8 + i at column
 // g, so a thread loads one contiguous run per key and ends with the 2 HD / 8
 // contiguous output dims from 2 t HD / 8 on.
 #pragma once
@@ -34,6 +34,17 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // tanh by 1 - 2 / (1 + e^2x): absolute error near 2^-23
 __device__ __forceinline__ float tanh_fast(float x) {
   return fmaf(-2.f, rcp_approx(1.f + ex2(2.f * KVQ_LOG2E * x)), 1.f);
+}
+// tanh to about 2 ulp without a branch: its Taylor polynomial below 0.35,
+// (1 - e^-2|x|) / (1 + e^-2|x|) above
+__device__ __forceinline__ float tanh_f32(float x) {
+  const float s = x * x, t = ex2(-2.f * KVQ_LOG2E * fabsf(x));
+  float c = fmaf(s, -1382.f / 155925.f, 62.f / 2835.f);
+  c = fmaf(s, c, -17.f / 315.f);
+  c = fmaf(s, c, 2.f / 15.f);
+  c = fmaf(s, c, -1.f / 3.f);
+  const float far = copysignf((1.f - t) * rcp_approx(1.f + t), x);
+  return fabsf(x) < 0.35f ? fmaf(x * s, c, x) : far;
 }
 // 8 x 8 fp16 tile: (row g, columns 2t, 2t + 1) per lane -> (column g, rows 2t, 2t + 1)
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -88,11 +99,6 @@ struct KvqFrag {
   static constexpr int NT = HD / 8;         // n-tiles of p . v = dims per thread and key
   static constexpr int VW = NT * BITS / 32; // 32-bit words of V codes per thread and key
 
-  // dim of k-index e (0..3) of step kk for thread t
-  __device__ static __forceinline__ int dim_of(int t, int kk, int e) {
-    if constexpr (BITS == 8) return ((kk >> 2) * 4 + t) * 16 + (kk & 3) * 4 + e;
-    else return t * (HD / 4) + (kk >> 1) * 8 + 2 * (kk & 1) + (e >> 1) + 4 * (e & 1);
-  }
   // q[kk][e] of a row from its head_dim values at src (16-byte aligned): the
   // thread's runs of consecutive dims by 16-byte loads
   template <typename T>
