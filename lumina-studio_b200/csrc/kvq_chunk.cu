@@ -965,65 +965,74 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
         }
         pair_bar();
         if (last_s) {
-          // Rows' largest reference and sums first (the Q tiles are free),
-          // then 4 dims of four rows per thread and pass, the parts in order;
-          // eight lanes hold neighbouring rows, four neighbouring dims.
+          // The parts' weights of each row first (the Q tiles are free), then
+          // 8 dims of two rows per thread and pass, the parts in order; eight
+          // lanes hold neighbouring rows, four neighbouring dims.
+          constexpr int WT = C::Q_BYTES / (4 * 256) - 2;  // parts whose weights fit; those of further ones are found anew
           const int np = ce - cb + 1;
           float2* stat = reinterpret_cast<float2*>(sm);
+          float* wt = reinterpret_cast<float*>(stat + 256);  // [part][256 rows]
           auto stat_of = [&](int p) { return reinterpret_cast<const float2*>(a.ws + slot_of(p) * part + (size_t)BM * HD); };
+          auto weight = [](float2 rl, float M) { return rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M); };
           if (tid < x.rows) {
             float M = -INFINITY, L = 0.f;
-#pragma unroll 8
+#pragma unroll 4
             for (int p = 0; p < np; ++p) M = fmaxf(M, __ldcg(stat_of(p) + tid).x);
-#pragma unroll 8
+#pragma unroll 4
             for (int p = 0; p < np; ++p) {
               const float2 rl = __ldcg(stat_of(p) + tid);
-              L += rl.y * (rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M));
+              const float w = weight(rl, M);
+              L += rl.y * w;
+              if (p < WT) wt[p * 256 + tid] = w;
             }
             stat[tid] = make_float2(M, L);
           }
           pair_bar();
-          constexpr int K = 4;
-          const int octets = (x.rows + 7) / 8;  // items: (octet, four dims' quad, lane)
-          for (int i0 = tid; i0 < octets * (HD / 16) * 32; i0 += 256 * K) {
-            int r[K], d4[K];
-            float4 y[K];
+          constexpr int K = 2, GROUPS = HD / 32;
+          const int octets = (x.rows + 7) / 8;  // items: (octet of rows, group of 32 dims, lane)
+          for (int i0 = tid; i0 < octets * GROUPS * 32; i0 += 256 * K) {
+            int r[K], d8[K];
+            bool there[K];
+            float4 y[K][2];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-              const int i = (i0 + 256 * k) >> 5, q = i / octets;
-              r[k] = (i - q * octets) * 8 + (lane & 7);
-              d4[k] = 4 * q + (lane >> 3);
-              if (q >= HD / 16 || r[k] >= x.rows) r[k] = -1;
-              y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              const int i = (i0 + 256 * k) >> 5, o = i / GROUPS;
+              r[k] = o * 8 + (lane & 7);
+              d8[k] = 4 * (i - o * GROUPS) + (lane >> 3);
+              there[k] = r[k] < x.rows;
+              if (!there[k]) r[k] = 0;
+              y[k][0] = y[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll 2
             for (int p = 0; p < np; ++p) {
               const float4* at_p = reinterpret_cast<const float4*>(a.ws + slot_of(p) * part);
 #pragma unroll
               for (int k = 0; k < K; ++k) {
-                if (r[k] < 0) continue;
-                const float2 rl = __ldcg(stat_of(p) + r[k]);
-                const float4 z = __ldcg(at_p + d4[k] * BM + r[k]);
-                const float w = rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - stat[r[k]].x);
-                y[k].x = fmaf(z.x, w, y[k].x); y[k].y = fmaf(z.y, w, y[k].y);
-                y[k].z = fmaf(z.z, w, y[k].z); y[k].w = fmaf(z.w, w, y[k].w);
+                const float w = p < WT ? wt[p * 256 + r[k]] : weight(__ldcg(stat_of(p) + r[k]), stat[r[k]].x);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float4 z = __ldcg(at_p + (2 * d8[k] + h) * BM + r[k]);
+                  y[k][h].x = fmaf(z.x, w, y[k][h].x); y[k][h].y = fmaf(z.y, w, y[k][h].y);
+                  y[k][h].z = fmaf(z.z, w, y[k][h].z); y[k][h].w = fmaf(z.w, w, y[k][h].w);
+                }
               }
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-              if (r[k] < 0) continue;
-              const float L = stat[r[k]].y, inv = 1.0f / L;
-              float4 o = y[k];
-              if (L == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-              else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+              if (!there[k]) continue;
+              const float L = stat[r[k]].y, inv = L == 0.f ? 0.f : 1.0f / L;
+              const bool none = L == 0.f;
+              float o[8] = {y[k][0].x, y[k][0].y, y[k][0].z, y[k][0].w, y[k][1].x, y[k][1].y, y[k][1].z, y[k][1].w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = none ? 0.f : o[e] * inv;
               const int packed = x.row0 + r[k], li2 = packed / a.G;
-              T* dst = static_cast<T*>(a.out) + (size_t)(x.first + li2) * a.ldo + (size_t)(x.kvh * a.G + packed - li2 * a.G) * HD;
-              if constexpr (BITS == 4) {
-                // columns 4 d4 .. + 3 hold dims b + {0, 4, 1, 5} or b + {2, 6, 3, 7}
-                const int b = (d4[k] >> 1) * 8 + 2 * (d4[k] & 1);
-                dst[b] = (T)o.x; dst[b + 4] = (T)o.y; dst[b + 1] = (T)o.z; dst[b + 5] = (T)o.w;
+              T* dst = static_cast<T*>(a.out) + (size_t)(x.first + li2) * a.ldo + (size_t)(x.kvh * a.G + packed - li2 * a.G) * HD + 8 * d8[k];
+              if constexpr (BITS == 4) {  // dim d of a group of 8 sits at column 2 (d & 3) + (d >> 2)
+                kvq_store4(dst, o[0], o[2], o[4], o[6]);
+                kvq_store4(dst + 4, o[1], o[3], o[5], o[7]);
               } else {
-                kvq_store4(dst + 4 * d4[k], o.x, o.y, o.z, o.w);
+                kvq_store4(dst, o[0], o[1], o[2], o[3]);
+                kvq_store4(dst + 4, o[4], o[5], o[6], o[7]);
               }
             }
           }
