@@ -30,11 +30,15 @@ int attend_launch(AttendArgs a, cudaStream_t s) {
   const int most = KVQ_DECODE_BLOCKS * KVQ_DECODE_ROWS;
   const int rows = max_packed <= 8 || (max_packed > most && a.G <= 8) ? 8 : KVQ_DECODE_ROWS;  // of a decode block
   a.few = a.G <= rows ? KVQ_DECODE_BLOCKS * rows : 0;
-  if (a.few && (max_packed <= a.few || !equal)) {
+  const bool decode = a.few && (max_packed <= a.few || !equal);
+  if (decode) {
     const int rc = kvq_decode_launch<HD, BITS, T>(a, rows, s);
     if (rc) return rc;
   }
-  return max_packed <= a.few ? LUMINA_OK : kvq_chunk_launch<HD, BITS, T>(a, s);
+  if (max_packed <= a.few) return LUMINA_OK;
+  a.tickets += KVQ_WS_DECODE_TICKETS;
+  a.ws += KVQ_WS_DECODE;
+  return kvq_chunk_launch<HD, BITS, T>(a, decode, s);
 }
 
 }  // namespace

@@ -33,21 +33,23 @@ struct AttendArgs {
 template <int HD, int BITS, typename T>
 int kvq_decode_launch(AttendArgs a, int rows, cudaStream_t s);
 
-// sequences of more than a.few packed rows (kvq_chunk.cu)
+// sequences of more than a.few packed rows (kvq_chunk.cu). beside: the decode
+// kernel was launched just before, and this one may start while it runs
 template <int HD, int BITS, typename T>
-int kvq_chunk_launch(AttendArgs a, cudaStream_t s);
+int kvq_chunk_launch(AttendArgs a, bool beside, cudaStream_t s);
 
 constexpr int KVQ_MAX_BLOCKS = 2048;  // row blocks whose key tiles the chunk kernel lines up
 constexpr int KVQ_CHUNK_CTAS = 160;   // CTAs of the chunk kernel at most
 constexpr int KVQ_CHUNK_ROWS = 256;   // packed rows of its partial states
 
-// workspace: tickets, then partial states
-constexpr size_t KVQ_WS_TICKETS = 4 * KVQ_MAX_CTAS * sizeof(int);
-inline size_t kvq_ws_bytes() {
-  const size_t decode = (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2) * 4;
-  const size_t chunk = (size_t)KVQ_CHUNK_CTAS * 2 * KVQ_CHUNK_ROWS * (128 + 2) * 4;
-  return KVQ_WS_TICKETS + (decode > chunk ? decode : chunk);
-}
+// workspace: tickets, then partial states; the two kernels of a mixed batch
+// overlap, so each has its own of both
+constexpr size_t KVQ_WS_DECODE_TICKETS = 4 * KVQ_MAX_CTAS, KVQ_WS_CHUNK_TICKETS = 2 * KVQ_CHUNK_CTAS;
+constexpr size_t KVQ_WS_TICKETS = (KVQ_WS_DECODE_TICKETS + KVQ_WS_CHUNK_TICKETS) * sizeof(int);
+constexpr size_t KVQ_WS_DECODE = (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2);  // floats
+constexpr size_t KVQ_WS_CHUNK = (size_t)KVQ_CHUNK_CTAS * 2 * KVQ_CHUNK_ROWS * (128 + 2);
+constexpr size_t kvq_ws_bytes() { return KVQ_WS_TICKETS + (KVQ_WS_DECODE + KVQ_WS_CHUNK) * sizeof(float); }
+static_assert(KVQ_WS_TICKETS % 16 == 0 && KVQ_WS_DECODE % 4 == 0, "16-byte aligned partial states");
 
 // rows of sequence s as the batch says (0 where row_start is out of order)
 __device__ __forceinline__ int kvq_seq_rows(const KvqView& v, int s, int& first, bool report = true) {

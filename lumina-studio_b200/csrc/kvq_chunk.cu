@@ -33,10 +33,10 @@
 //
 // Bound by the softmax warps, whose pass over a tile takes longer than the
 // products it overlaps. 2048 rows behind 14K cached tokens, 32 / 8 heads of
-// 128, int8, fp16 rows: 835 us, 617 TFLOP/s (0.37 of the bf16 peak). The
+// 128, int8, fp16 rows: 822 us, 625 TFLOP/s (0.38 of the bf16 peak). The
 // loops' code size matters: the same with its helpers inline, twice the text,
 // was 10 % slower. 285 rows of 28 / 4 heads of 64 over 4096 int4 keys, fp32
-// rows with cap, distance bias, window and prefix: 68 us.
+// rows with cap, distance bias, window and prefix: 63 us.
 //
 // Waits are bounded: one that gives up sets bit 5 of the device fault word,
 // every role leaves its loop, and the CTA frees its tensor memory and exits.
@@ -1050,28 +1050,48 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
     ck_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+  // the call's decode kernel, if any, has ended too when this one ends
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace
 
 template <int HD, int BITS, typename T>
-int kvq_chunk_launch(AttendArgs a, cudaStream_t s) {
+int kvq_chunk_launch(AttendArgs a, bool beside, cudaStream_t s) {
   using C = CkCfg<HD>;
   auto kern = a.cap > 0.f || a.slopes ? kvq_chunk_kernel<HD, BITS, T, false> : kvq_chunk_kernel<HD, BITS, T, true>;
   a.min_cells = 2;
   const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_chunk");
   if (rc) return rc;
-  kern<<<min(sm_count(), KVQ_CHUNK_CTAS), CK_THREADS, C::SMEM + (size_t)a.v.n_seq * 4, s>>>(a);
-  LUMINA_LAUNCH_CHECK();
+  // Beside a decode kernel: it lets this one start as its CTAs leave, and this
+  // one's end waits for it. Nothing passes between the two (workspaces and
+  // outputs are apart), and what came before it ended before it began.
+  // 317 rows of 17 sequences, one of them for this kernel: 82 us, 88 in turn.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(min(sm_count(), KVQ_CHUNK_CTAS));
+  cfg.blockDim = dim3(CK_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM + (size_t)a.v.n_seq * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = beside ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("kvq_chunk launch: %s", cudaGetErrorString(e));
+    return LUMINA_E_CUDA;
+  }
   return LUMINA_OK;
 }
-template int kvq_chunk_launch<128, 8, __half>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<128, 8, float>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<128, 4, __half>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<128, 4, float>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<64, 8, __half>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<64, 8, float>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<64, 4, __half>(AttendArgs, cudaStream_t);
-template int kvq_chunk_launch<64, 4, float>(AttendArgs, cudaStream_t);
+template int kvq_chunk_launch<128, 8, __half>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<128, 8, float>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<128, 4, __half>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<128, 4, float>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<64, 8, __half>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<64, 8, float>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<64, 4, __half>(AttendArgs, bool, cudaStream_t);
+template int kvq_chunk_launch<64, 4, float>(AttendArgs, bool, cudaStream_t);
 
 }  // namespace lumina

@@ -83,6 +83,8 @@ kvq_decode_kernel(AttendArgs a) {
   // of a score at most, below the fp16 rounding of p). fp32 rows use exact
   // signed codes and split q and p.
   constexpr bool FAST = !F32, IK = FAST && BITS == 8, OFFSET = FAST && BITS == 4;
+  // a chunk kernel of the same call may take the SMs that this one leaves
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint8_t sm[];
   float* slab = reinterpret_cast<float*>(sm);
   int* cells = reinterpret_cast<int*>(sm + C::SMEM);  // inclusive prefix of cells over sequences

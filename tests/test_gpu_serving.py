@@ -408,6 +408,59 @@ def test_decode_step_in_a_graph(sv):
             assert rel(got[s:s + 1], want) < TOL["float16"]
 
 
+@pytest.mark.parametrize("io", ["float16", "float32"])
+def test_mixed_batches_in_a_row(sv, io):
+    """A chunk beside decoding rows, writes and attention in turn on one
+    stream and as a captured graph: each step sees the one before whole, and
+    repeats bit for bit."""
+    import torch
+    rng = np.random.default_rng(21)
+    hd, page, heads, n_kv = 64, 16, 8, 2
+    dt = getattr(torch, io)
+    rows, lens = [1] * 20 + [150, 1, 30], rng.integers(200, 3000, 23).tolist()
+    n = sum(rows)
+    table, n_pages, _ = layout(rng, lens, page)
+    start = dev(random_pool(rng, n_pages, n_kv, 8, hd, page))
+    pool = sv.KVPool(start.clone(), 8, hd, page)
+    batch = batch_of(sv, rows, lens, table)
+    cos, sin = (dev(f(np.arange(3000)[:, None] * np.linspace(1, 0.01, hd // 2)[None]).astype(np.float32)) for f in (np.cos, np.sin))
+    x0 = dev(rng.standard_normal((n, (heads + 2 * n_kv) * hd)).astype(np.float32), dt)
+    x, q, out = x0.clone(), torch.empty(n, heads, hd, device="cuda", dtype=dt), torch.empty(n, heads, hd, device="cuda", dtype=dt)
+    ws = sv.attend_workspace(0)
+
+    def step():  # the output feeds the next step's q, k and v
+        pool.append(batch, x[:, :heads * hd], x[:, heads * hd:(heads + n_kv) * hd], x[:, (heads + n_kv) * hd:], cos, sin, out=q)
+        pool.attend(batch, q, out=out, workspace=ws)
+        x[:, :heads * hd] += out.flatten(1)
+        x[:, heads * hd:] += out.flatten(1)[:, :2 * n_kv * hd]
+
+    def reset():
+        x.copy_(x0)
+        pool.data.copy_(start)
+
+    reset()
+    outs = []
+    for _ in range(3):
+        step()
+        torch.cuda.synchronize()
+        outs.append(out.clone())
+    k, v = ref.rows_of(pool.data.cpu().numpy(), table[20], lens[20], 8, hd, page)
+    want = ref.attend(q[20:170].double().cpu().numpy(), k, v, lens[20], hd ** -0.5)
+    assert rel(out[20:170].double().cpu().numpy(), want) < TOL[io]
+    reset()
+    for _ in range(3):  # without a wait between them
+        step()
+    assert torch.equal(out, outs[-1])
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        step()
+    reset()
+    for i in range(3):
+        g.replay()
+        assert torch.equal(out, outs[i])
+
+
 def test_two_streams_two_workspaces(sv):
     import torch
     rng = np.random.default_rng(8)
