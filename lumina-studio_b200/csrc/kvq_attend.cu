@@ -3,15 +3,17 @@
 //
 // A sequence of few packed rows (new rows x query heads per KV head) is bound
 // by its cache's bytes and goes to the decode kernel (kvq_decode.cu), in up to
-// four tasks of 16 rows per KV head; one of more rows is bound by the tensor
-// pipe and goes to the chunk kernel (kvq_chunk.cu). Each kernel takes its own
-// sequences out of the batch, so a batch may mix them. Decode / chunk kernel,
-// int8, head dim 128, 8 KV heads, lengths up to 4096:
-//   8 sequences,  20 packed rows    37 /  58 us
-//   8 sequences,  64 packed rows    58 /  66 us
-//   8 sequences, 128 packed rows    96 /  80 us
-//   32 sequences, 32 packed rows    95 / 136 us
-//   32 sequences, 64 packed rows   172 / 146 us
+// three (fp32 rows: four) tasks of 16 rows per KV head; one of more rows goes
+// to the chunk kernel (kvq_chunk.cu), bound by its tensor and softmax work.
+// Each kernel takes its own sequences out of the batch, so a batch may mix
+// them. Decode / chunk kernel, int8, head dim 128, 8 KV heads, lengths up to
+// 4096, fp16 rows unless said:
+//   8 sequences,  20 packed rows     38 /  56 us
+//   8 sequences,  64 packed rows     57 /  58 us, fp32 rows 64 / 75 us
+//   32 sequences, 32 packed rows     95 / 128 us
+//   32 sequences, 64 packed rows    171 / 133 us
+// Sequences for the decode kernel take at least a cell per warp and CTA
+// (1 x 640 tokens, 32 KV heads: 12.3 us; 14.4 with two cells, 16.4 with three).
 // Beside a sequence for the chunk kernel the others mostly bring one row, so
 // the decode kernel's blocks are 8 rows there.
 #include <cmath>
@@ -27,9 +29,10 @@ int attend_launch(AttendArgs a, cudaStream_t s) {
   // a batch of equal row counts needs one of the two kernels only
   const long long max_packed = (long long)a.v.max_rows * a.G;
   const bool equal = (long long)a.v.max_rows * a.v.n_seq == a.v.n_rows;
-  const int most = KVQ_DECODE_BLOCKS * KVQ_DECODE_ROWS;
+  const int blocks = sizeof(T) == 4 ? KVQ_DECODE_BLOCKS : KVQ_DECODE_BLOCKS - 1;
+  const int most = blocks * KVQ_DECODE_ROWS;
   const int rows = max_packed <= 8 || (max_packed > most && a.G <= 8) ? 8 : KVQ_DECODE_ROWS;  // of a decode block
-  a.few = a.G <= rows ? KVQ_DECODE_BLOCKS * rows : 0;
+  a.few = a.G <= rows ? blocks * rows : 0;
   const bool decode = a.few && (max_packed <= a.few || !equal);
   if (decode) {
     const int rc = kvq_decode_launch<HD, BITS, T>(a, rows, s);
@@ -91,7 +94,7 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
   a.slopes = args->slopes_dev;
   a.prefix = args->prefix_dev;
   a.window = args->window;
-  a.min_cells = 8;
+  a.min_cells = 4;
   a.tickets = static_cast<int*>(args->workspace_dev);
   a.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(args->workspace_dev) + KVQ_WS_TICKETS);
   a.spin = wait_spin_limit();
