@@ -94,7 +94,6 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
   a.slopes = args->slopes_dev;
   a.prefix = args->prefix_dev;
   a.window = args->window;
-  a.min_cells = 4;
   a.tickets = static_cast<int*>(args->workspace_dev);
   a.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(args->workspace_dev) + KVQ_WS_TICKETS);
   a.spin = wait_spin_limit();

@@ -23,7 +23,6 @@ struct AttendArgs {
   const int* prefix;
   int window;
   int few;        // sequences of up to this many packed rows (rows x G) are the decode kernel's
-  int min_cells;  // decode: cells per CTA at least
   float* ws;      // partial states
   int* tickets;   // two per partial state, zero between launches
   long long spin;

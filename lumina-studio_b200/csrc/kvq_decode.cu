@@ -143,7 +143,7 @@ kvq_decode_kernel(AttendArgs a) {
     return;
   }
   const unsigned Tn = (unsigned)T_all, U = Tn * (unsigned)v.n_kv;
-  const unsigned share = max((U + gridDim.x - 1) / gridDim.x, (unsigned)a.min_cells);
+  const unsigned share = max((U + gridDim.x - 1) / gridDim.x, (unsigned)W);  // a cell per warp
   const unsigned u0 = blockIdx.x * share, u1 = min(U, u0 + share);
   if (u0 >= U) return;
 
