@@ -23,7 +23,8 @@
 //
 // Measured: 64 sequences of up to 8192 tokens, 32 / 8 heads of 128, int8, fp16
 // rows: 87 us, 0.71 of the copy rate; 2 sequences of up to 131072, 32 / 4
-// heads, int4: 60 us, bound by instruction issue (about 600 per cell); one of
+// heads, int4: 60 us, bound by the chain of a cell's math (two warps per
+// scheduler issue 0.3 instructions a cycle; about 600 per cell); one of
 // 640 tokens, 32 / 32 heads, fp32 rows: 12.3 us. CTAs of four warps, two per SM:
 // one merges and joins while the other streams. A third CTA per SM spills at
 // head dim 128 (the 64 sequences: 118 us).
