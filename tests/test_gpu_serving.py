@@ -650,6 +650,22 @@ def test_no_rows(sv):
 # ---------------------------------------------------------------------------
 # logits
 # ---------------------------------------------------------------------------
+def test_logits_offsets_stay_within_the_lists(sv):
+    """Offsets before, past and out of order: the lists' own entries count,
+    a reversed range is empty."""
+    import torch
+    x = dev(np.linspace(1, 2, 3 * 40, dtype=np.float32).reshape(3, 40))
+    toks, vals = dev(np.arange(6, dtype=np.int32)), dev(np.full(6, 8.0, np.float32))
+    two = torch.full((3,), 2.0, device="cuda")
+    offs = dev(np.array([-7, 1 << 30, 2, 4], np.int32))  # rows: all six, none, tokens 2 and 3
+    got, _ = sv.adjust_logits(x, history=(offs, toks), repeat=two, bias=(offs, toks, vals))
+    want = x.clone()
+    for row, named in ((0, range(6)), (2, (2, 3))):
+        for t in named:
+            want[row, t] = want[row, t] / 2 + 8
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("rows,vocab,hist,biases,masked,pad", [
     (1, 1, 0, 0, False, 0),
     (1, 32000, 64, 5, True, 0),
