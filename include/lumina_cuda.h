@@ -344,7 +344,8 @@ typedef struct {
  * length or page number out of range sets bit 64 of the device fault word
  * (lumina_fault_status); append and read skip the rows it concerns, attend
  * leaves the rows of that sequence unspecified and serves the others. Pages
- * that no token below len lies on may hold any number. */
+ * that no token below len lies on may hold any number. pages_ld * page_size +
+ * n_rows is at most 2^31 - 256. */
 typedef struct {
   const int* row_start_dev; /* n_seq + 1 */
   const int* len_dev;       /* n_seq */
@@ -403,7 +404,7 @@ typedef struct {
   float softcap;           /* 0: none */
   const float* slopes_dev; /* n_heads, or NULL */
   const int* prefix_dev;   /* n_seq, or NULL */
-  int window;              /* 0: unlimited */
+  int window;              /* 0, or no less than the page table's tokens: unlimited */
   void* workspace_dev;
   size_t workspace_bytes;
 } lumina_kvq_attend_args;

@@ -93,7 +93,9 @@ int lumina_kvq_attend(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch
   a.cap = args->softcap;
   a.slopes = args->slopes_dev;
   a.prefix = args->prefix_dev;
-  a.window = args->window;
+  // no shorter than the cache: it hides nothing (and a position less the
+  // window stays within an int)
+  a.window = args->window >= (long long)batch->pages_ld * pool->page_size ? 0 : args->window;
   a.tickets = static_cast<int*>(args->workspace_dev);
   a.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(args->workspace_dev) + KVQ_WS_TICKETS);
   a.spin = wait_spin_limit();

@@ -34,8 +34,9 @@ int kvq_view(const lumina_kvq_pool* p, const lumina_kvq_batch* b, const char* wh
                    "%s: page size %d, one of 16, 32, 64, 128", what, p->page_size);
   LUMINA_CHECK_ARG(b->n_seq >= 1 && b->n_seq <= KVQ_MAX_SEQ, "%s: %d sequences, 1..%d", what, b->n_seq, KVQ_MAX_SEQ);
   LUMINA_CHECK_ARG(b->pages_ld >= 1, "%s: pages_ld %d", what, b->pages_ld);
-  LUMINA_CHECK_ARG((long long)b->pages_ld * p->page_size < (1LL << 31), "%s: page table of %d pages of %d tokens", what,
-                   b->pages_ld, p->page_size);
+  // positions from -n_rows to the end of the last key tile are ints
+  LUMINA_CHECK_ARG((long long)b->pages_ld * p->page_size + max(0, b->n_rows) <= (1LL << 31) - 256,
+                   "%s: page table of %d pages of %d tokens beside %d rows", what, b->pages_ld, p->page_size, b->n_rows);
   LUMINA_CHECK_ARG(b->n_rows >= 0 && b->max_rows >= 0 && b->max_rows <= b->n_rows &&
                        (long long)b->max_rows * b->n_seq >= b->n_rows,
                    "%s: %d rows of at most %d in %d sequences", what, b->n_rows, b->max_rows, b->n_seq);

@@ -1,0 +1,80 @@
+"""Edges of the quantized-page attention and of its calls on a B200: values
+of very different sizes, outlier dims, NaN behind vanishing weights, waits
+that give up, captured graphs, ranges. Helpers and base tolerances are those of
+test_gpu_serving.py."""
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from test_gpu_serving import TOL, batch_of, check_attend, dev, layout, no_fault, random_pool, rel, run_attend, sv  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def pool_of(rng, k, v, bits, page):
+    """One sequence's K and V rows (tokens, n_kv, hd) quantized into shuffled
+    pages: (pool bytes, page table (1, n))."""
+    ln, n_kv, hd = k.shape
+    table, n_pages, _ = layout(rng, [ln], page)
+    pool = random_pool(rng, n_pages, n_kv, bits, hd, page)
+    nb, top = hd * bits // 8, 127 if bits == 8 else 15
+    t = np.arange(ln)
+    pg, off = table[0, t // page], t % page
+    for i, x in enumerate((k, v)):
+        amax = np.maximum(np.abs(x).max(-1), 1e-30)
+        if bits == 8:
+            raw = np.rint(x * (127 / amax[..., None])).astype(np.int8).view(np.uint8)
+        else:
+            c = np.clip(np.rint(x * (7.5 / amax[..., None]) + 7.5), 0, 15).astype(np.uint8)
+            raw = c[..., 0::2] | (c[..., 1::2] << 4)
+        codes = pool[:, :, i * page * nb:(i + 1) * page * nb].reshape(n_pages, n_kv, page, nb)
+        codes[pg, :, off] = raw
+        pool[:, :, i * page * nb:(i + 1) * page * nb] = codes.reshape(n_pages, n_kv, page * nb)
+        set_scales(pool, bits, hd, page, i, pg, off, (amax / top).astype(np.float32))
+    return pool, table
+
+
+def set_scales(pool, bits, hd, page, which, pg, off, values):
+    """K (0) or V (1) scales of the tokens at (pg, off), (tokens, n_kv) or a number."""
+    a = 2 * page * (hd * bits // 8) + 4 * page * which
+    s = np.ascontiguousarray(pool[:, :, a:a + 4 * page]).view(np.float32)
+    s[pg, :, off] = values
+    pool[:, :, a:a + 4 * page] = s.view(np.uint8)
+
+
+def attend_both(sv, pool, table, bits, hd, page, q, ln, slopes=None, window=0, **kw):
+    """(result, float64 definition) of the last rows q (n, heads, hd) of one sequence."""
+    out = sv.KVPool(dev(pool), bits, hd, page).attend(
+        batch_of(sv, [q.shape[0]], [ln], table), q, window=window, slopes=None if slopes is None else dev(slopes), **kw)
+    k, v = ref.rows_of(pool, table[0], ln, bits, hd, page)
+    want = ref.attend(q.double().cpu().numpy(), k, v, ln, hd ** -0.5, 0.0,
+                      None if slopes is None else slopes.astype(np.float64), window)
+    return out.float().cpu().numpy(), want
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30, 1 << 20, 64, 63])
+@pytest.mark.parametrize("rows,lens", [([5], [2]), ([90, 3], [60, 1])])
+def test_windows_past_the_cache(sv, io, window, rows, lens):
+    """A window no shorter than the cache hides nothing, also beside rows
+    before the first token."""
+    got, want = run_attend(sv, 8, 64, io, 4, 2, 16, rows, lens, window=window, seed=81)
+    at = 0
+    for n, ln in zip(rows, lens):
+        assert (got[at:at + n - ln] == 0).all()
+        check_attend(got[at + n - ln:at + n], want[at + n - ln:at + n], io)
+        at += n
+
+
+def test_page_tables_past_int_positions(sv):
+    """Tokens of a page table and rows whose positions would pass 31 bits are refused."""
+    import torch
+    from lumina_b200.cuda import LuminaError
+    pool = sv.KVPool.empty(1, 1, 64, 8, 16)
+    batch = batch_of(sv, [1], [1], np.zeros((1, 1), np.int32))
+    batch.c.pages_ld = 2 ** 27 - 1  # 2^31 - 16 tokens
+    x = torch.zeros(1, 1, 64, device="cuda")
+    for call in (lambda: pool.attend(batch, x), lambda: pool.read(batch),
+                 lambda: pool.append(batch, x, x, x, x[0, :, :32], x[0, :, :32])):
+        with pytest.raises(LuminaError, match="page table"):
+            call()
