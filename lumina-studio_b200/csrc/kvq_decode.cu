@@ -182,6 +182,8 @@ kvq_decode_kernel(AttendArgs a) {
   segment(u0, ps);
   unsigned pu = u0;
   int pc = ps.lo + warp, pg[NK], pj = 0;
+#pragma unroll
+  for (int n = 0; n < NK; ++n) pg[n] = -2;  // a warp without a cell reads page 0 too
   const int* table = v.pages + (size_t)ps.s * v.pages_ld;
   const uint8_t* head = v.pool + (uint32_t)ps.kvh * v.block_bytes + k_lane;
   bool more = true;

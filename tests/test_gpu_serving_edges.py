@@ -78,3 +78,19 @@ def test_page_tables_past_int_positions(sv):
                  lambda: pool.append(batch, x, x, x, x[0, :, :32], x[0, :, :32])):
         with pytest.raises(LuminaError, match="page table"):
             call()
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd,page", [(128, 16), (64, 32), (64, 128)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_fewer_cells_than_warps(sv, io, bits, hd, page, rows):
+    """One key in a pool of one page: warps without a cell have a page of the
+    pool to read all the same, and nothing to add."""
+    import torch
+    rng = np.random.default_rng(85)
+    pool = random_pool(rng, 1, 1, bits, hd, page)
+    q = dev(rng.standard_normal((rows, 2, hd)).astype(np.float32), getattr(torch, io))
+    got, want = attend_both(sv, pool, np.zeros((1, 1), np.int32), bits, hd, page, q, 1)
+    assert (got[:-1] == 0).all()
+    check_attend(got[-1:], want[-1:], io)
