@@ -390,10 +390,12 @@ int lumina_kvq_read(const lumina_kvq_pool* pool, const lumina_kvq_batch* batch, 
  * least lumina_kvq_workspace_bytes, zeroed once by the caller before its
  * first use and left reusable by every call; calls that may overlap on the
  * GPU need workspaces of their own. The order of every sum is fixed by the
- * batch's lengths, so equal calls give equal bits. The sequences' lengths
- * times n_kv add up to less than 2^31 (bit 64 and no output otherwise). A wait inside
- * that gives up sets bit 32 and leaves outputs unwritten. At most 128 query
- * heads per KV head. */
+ * batch's lengths, so equal calls give equal bits. A sequence counts one for
+ * each 128 of its keys and 128 of its packed rows (new rows x n_heads / n_kv),
+ * or for each 16 of its keys and each new row where it has up to 64 packed
+ * rows; the counts times n_kv add up to less than 2^30 (bit 64 and no output
+ * otherwise). A wait inside that gives up sets bit 32 and leaves outputs
+ * unwritten. At most 128 query heads per KV head. */
 typedef struct {
   const void* q_dev;
   void* out_dev;

@@ -70,6 +70,11 @@ __device__ __forceinline__ void kvq_store4(__half* p, float a, float b, float c,
       make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
+// a + b for the prefix sums of the work lines, no further than KVQ_MANY (which
+// a + b of two such sums does not pass 32 bits for, and no line may reach)
+constexpr unsigned KVQ_MANY = 0x40000000u;
+__device__ __forceinline__ unsigned kvq_sum(unsigned a, unsigned b) { return min(a + b, KVQ_MANY); }
+
 // f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
 template <int N, int I = 0, typename Fn>
 __device__ __forceinline__ void static_for(Fn&& f) {

@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   int* blocks = line + KVQ_MAX_BLOCKS;                   // inclusive prefix of blocks over sequences
   __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, idle;
   __shared__ uint32_t tmem_s, skm_s[2][4], svm_s[2][4];  // a tile's largest K and V scale, one per warp that filled it
-  __shared__ int scan_s[CK_THREADS / 32], abort_s, last_s;
+  __shared__ unsigned scan_s[CK_THREADS / 32];
+  __shared__ int abort_s, last_s;
   __shared__ float m_s[128], l_s[128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const KvqView& v = a.v;
@@ -312,19 +313,19 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   }
 
   // ---- the line of key tiles
-  auto block_scan = [&](int x, int& total) {  // inclusive over the CTA; two barriers
-    int inc = x;
+  auto block_scan = [&](unsigned x, unsigned& total) {  // inclusive over the CTA; two barriers
+    unsigned inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-      const int y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+      const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc = kvq_sum(inc, y);
     }
     if (lane == 31) scan_s[warp] = inc;
     __syncthreads();
     total = 0;
     for (int w = 0; w < CK_THREADS / 32; ++w) {
-      if (w < warp) inc += scan_s[w];
-      total += scan_s[w];
+      if (w < warp) inc = kvq_sum(inc, scan_s[w]);
+      total = kvq_sum(total, scan_s[w]);
     }
     __syncthreads();
     return inc;
@@ -332,16 +333,17 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   int NBt = 0;
   for (int s0 = 0; s0 < v.n_seq; s0 += CK_THREADS) {
     const int s = s0 + tid;
-    int first, nb = 0, total;
+    int first, nb = 0;
+    unsigned total;
     if (s < v.n_seq) {
       const int n = kvq_seq_rows(v, s, first, blockIdx.x == 0);
       if ((long long)n * a.G > a.few) nb = (int)(((long long)n * a.G + BM - 1) / BM);
       const int len = __ldg(v.len + s);
       if (nb && (len < 0 || len > cap_tokens) && blockIdx.x == 0) kvq_fault(v, KVQ_FAULT_DATA);
     }
-    const int inc = block_scan(nb, total);
-    if (s < v.n_seq) blocks[s] = NBt + inc;
-    NBt += total;
+    const unsigned inc = block_scan(nb, total);
+    if (s < v.n_seq) blocks[s] = kvq_sum(NBt, inc);
+    NBt = kvq_sum(NBt, total);
   }
   __syncthreads();
   CkLine ln{a, line, blocks, 0, 0, 0u, 0u, 0u, false};
@@ -353,11 +355,11 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
     for (int b0 = 0; b0 < NBt; b0 += CK_THREADS) {
       CkSeg x;
       x.total = 0;
-      int total;
+      unsigned total;
       if (b0 + tid < NBt) ck_describe<BM>(ln, b0 + tid, x);
-      const int inc = block_scan(x.total, total);
-      if (b0 + tid < NBt) line[b0 + tid] = Tn + inc;
-      Tn += total;
+      const unsigned inc = block_scan(x.total, total);
+      if (b0 + tid < NBt) line[b0 + tid] = kvq_sum(Tn, inc);
+      Tn = kvq_sum(Tn, total);
     }
   }
   ck_fence_before();
@@ -365,8 +367,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   ck_fence_after();
   const uint32_t tmem = tmem_s;
   const long long U64 = (long long)Tn * v.n_kv;
-  const unsigned U = U64 > 0x3fffffffLL ? 0u : (unsigned)U64;
-  if (U64 > 0x3fffffffLL && tid == 0) kvq_fault(v, KVQ_FAULT_DATA);
+  const unsigned U = U64 >= KVQ_MANY ? 0u : (unsigned)U64;
+  if (U64 >= KVQ_MANY && tid == 0) kvq_fault(v, KVQ_FAULT_DATA);
   const unsigned share = whole ? 1u : max((U + gridDim.x - 1) / gridDim.x, 1u);  // (300 tokens x 285 rows: 29 us, 41 with two tiles at least)
   // units [u0, u1), or tasks u0, u0 + gridDim.x, ...
   const unsigned u0 = whole ? blockIdx.x : min(U, blockIdx.x * share), u1 = whole ? U : min(U, u0 + share);

@@ -90,7 +90,8 @@ kvq_decode_kernel(AttendArgs a) {
   float* slab = reinterpret_cast<float*>(sm);
   int* cells = reinterpret_cast<int*>(sm + C::SMEM);  // inclusive prefix of cells over sequences
   __shared__ float m_s[W][R], l_s[W][R], M_s[R], L_s[R];
-  __shared__ int scan_s[W], last_s;
+  __shared__ unsigned scan_s[W];
+  __shared__ int last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const KvqView& v = a.v;
   const int cap_tokens = v.pages_ld << v.page_shift;
@@ -123,11 +124,11 @@ kvq_decode_kernel(AttendArgs a) {
     Seg x;
     x.total = x.blocks = 0;
     if (s < v.n_seq) describe(s, x, blockIdx.x == 0);
-    int inc = x.total * x.blocks;
+    unsigned inc = (unsigned)min((long long)x.total * x.blocks, (long long)KVQ_MANY);
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-      const int y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+      const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc = kvq_sum(inc, y);
     }
     if (lane == 31) scan_s[warp] = inc;
     __syncthreads();
@@ -139,7 +140,7 @@ kvq_decode_kernel(AttendArgs a) {
     if (s < v.n_seq) cells[s] = (int)(before + inc);
     __syncthreads();
   }
-  if (T_all == 0 || T_all * v.n_kv > 0x3fffffffLL) {
+  if (T_all == 0 || T_all * v.n_kv >= KVQ_MANY) {
     if (T_all && tid == 0) kvq_fault(v, KVQ_FAULT_DATA);
     return;
   }

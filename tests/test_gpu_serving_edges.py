@@ -94,3 +94,19 @@ def test_fewer_cells_than_warps(sv, io, bits, hd, page, rows):
     got, want = attend_both(sv, pool, np.zeros((1, 1), np.int32), bits, hd, page, q, 1)
     assert (got[:-1] == 0).all()
     check_attend(got[-1:], want[-1:], io)
+
+
+@pytest.mark.parametrize("io,heads,rows", [("float32", 16, 4), ("float16", 128, 64)])
+def test_work_past_the_lines_of_tiles(sv, io, heads, rows):
+    """32 sequences of 2^28 tokens with several row blocks each: 2^31 cells or
+    key tiles, which an int does not count. Reported, nothing is written."""
+    import torch
+    from lumina_b200 import cuda
+    n, page, hd = 32, 128, 64 if io == "float16" else 128
+    pool = sv.KVPool.empty(1, 1, hd, 8, page)
+    pages = torch.zeros(n, 2 ** 21, dtype=torch.int32, device="cuda")
+    batch = sv.SeqBatch(dev(np.arange(0, n * rows + 1, rows, dtype=np.int32)), dev(np.full(n, 2 ** 28, np.int32)), pages, n * rows, rows)
+    out = torch.full((n * rows, heads, hd), 77.0, device="cuda", dtype=getattr(torch, io))
+    pool.attend(batch, torch.zeros_like(out), out=out)
+    assert cuda.fault_status(0) == sv.FAULT_DATA
+    assert (out == 77.0).all()
