@@ -427,7 +427,7 @@ typedef struct {
   const float* logits_dev;
   float* out_dev;
   int ld, ldo;
-  int rows, vocab;
+  int rows, vocab;            /* below 2^24, up to 2^30 */
   const int* hist_start_dev;  /* rows + 1 offsets into hist_tok, or NULL */
   const int* hist_tok_dev;
   int hist_len;               /* tokens in hist_tok: offsets are kept within 0..hist_len */

@@ -229,7 +229,9 @@ using namespace lumina;
 extern "C" int lumina_logits_adjust(const lumina_logits_args* args, void* stream) {
   LUMINA_CHECK_ARG(args, "logits_adjust: null arguments");
   const lumina_logits_args a = *args;
-  LUMINA_CHECK_ARG(a.rows >= 0 && a.vocab >= 1 && a.rows < (1 << 24), "logits_adjust: %d rows x %d", a.rows, a.vocab);
+  // tokens plus a chunk of them stay within an int
+  LUMINA_CHECK_ARG(a.rows >= 0 && a.vocab >= 1 && a.rows < (1 << 24) && a.vocab <= (1 << 30), "logits_adjust: %d rows x %d",
+                   a.rows, a.vocab);
   if (a.rows == 0) return LUMINA_OK;
   LUMINA_CHECK_ARG(a.logits_dev && a.out_dev, "logits_adjust: null pointer");
   LUMINA_CHECK_ARG(a.ld >= a.vocab && a.ldo >= a.vocab, "logits_adjust: ld %d / ldo %d smaller than %d", a.ld, a.ldo, a.vocab);

@@ -79,3 +79,11 @@ def test_the_plain_attention_by_differences():
         w[j] += 1.0
         moved = np.abs(ref.attend(q, k, w, ln, 0.5, window=window, prefix=pre) - base).max(axis=(1, 2)) > 1e-9
         assert moved.tolist() == [j < pre or (p - window < j <= p) for p in range(ln - n, ln)]
+
+
+def test_vocabularies_past_int_tokens_are_refused():
+    """Before any GPU work: a token plus a chunk of tokens would pass 31 bits."""
+    lib = cuda.bound_lib()
+    a = serving._Logits(16, 16, 2 ** 31 - 1, 2 ** 31 - 1, 1, 2 ** 30 + 1)
+    assert lib.lumina_logits_adjust(ctypes.byref(a), None) == 1
+    assert str(2 ** 30 + 1) in cuda.last_error(lib)
