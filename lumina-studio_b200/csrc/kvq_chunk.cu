@@ -22,9 +22,10 @@
 // always for fp32 rows) both softmax groups hold the SAME rows and take
 // alternate key tiles, and merge at the end.
 //
-// The reference exponent of a row (its maximum and the exponent of the V
-// scales) moves only when P might leave fp16's range or a V scale passes its
-// exponent; only then O is rescaled in tensor memory.
+// A row's reference is its own largest score times value scale (P has to fit
+// fp16, and a key that the row does not see, or hardly, takes nothing from the
+// others). It moves only when P might leave fp16's range; only then O is
+// rescaled in tensor memory.
 //
 // The key tiles of all tasks form one line that the CTAs share evenly; tasks
 // that span CTAs leave partial states in the workspace, joined in part order
@@ -54,12 +55,15 @@ namespace {
 constexpr int CK_KEYS = 128;                // keys per tile
 constexpr int CK_DEQ = 8, CK_MMA = 12;      // first warp of the roles
 constexpr int CK_THREADS = 32 * (CK_MMA + 1);
-// P is 2^LIFT at the maximum the reference was set by, and may grow to 2^15
-// (fp16's range) before the reference moves. fp32 rows need their small p's
-// low parts above fp16's subnormals, fp16 rows a rarely moving reference.
+// P is about 2^LIFT at the key the reference was set by, and may grow to 2^15
+// (fp16's range) before the reference moves. fp16 leaves a P (fp32 rows: its
+// low part) an error of 2^-25 at least, which n keys add up to 2^-25 sqrt(n):
+// at 128K keys 3e-5 of the largest P V for fp16 rows, 2e-7 for fp32 rows. A
+// wide margin saves exact maxima (2048 rows behind 14K tokens: 838 us with
+// LIFT 0, 823 with -2; fp32 rows, 1024 behind 7K: 429 us with 10, 415 with 5).
 template <bool F32>
 struct CkLift {
-  static constexpr float LIFT = F32 ? 10.f : 4.f, MARGIN = 15.f - LIFT;
+  static constexpr float LIFT = F32 ? 5.f : -2.f, MARGIN = 15.f - LIFT;
 };
 constexpr int CK_TILE = 128 * 128;          // bytes of a [128 rows][64 fp16] block
 constexpr uint32_t CK_S = 0, CK_O = 256;    // tensor memory columns: S tiles, O tiles, 128 apart
@@ -70,7 +74,7 @@ struct CkCfg {
   static constexpr int BYTES = BLKS * CK_TILE;       // one K, V or Q tile
   static constexpr int Q_BYTES = 2 * 128 * HD * 2 > 128 * HD * 4 ? 2 * 128 * HD * 2 : 128 * HD * 4;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * BYTES, OFF_SC = OFF_V + 2 * BYTES;
-  static constexpr int OFF_LINE = OFF_SC + 2 * 2 * CK_KEYS * 4;  // [stage][K | V scale][key]
+  static constexpr int OFF_LINE = OFF_SC + 2 * 3 * CK_KEYS * 4;  // [stage][K scale | V scale | its size (kvq_size)][key]
   static constexpr size_t SMEM = OFF_LINE + (size_t)KVQ_MAX_BLOCKS * 4 + 1024;  // + n_seq ints
 };
 
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   int* line = reinterpret_cast<int*>(sm + C::OFF_LINE);  // inclusive prefix of tiles over blocks
   int* blocks = line + KVQ_MAX_BLOCKS;                   // inclusive prefix of blocks over sequences
   __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, idle;
-  __shared__ uint32_t tmem_s, skm_s[2][4], svm_s[2][4];  // a tile's largest K and V scale, one per warp that filled it
+  __shared__ uint32_t tmem_s;
+  __shared__ __align__(8) float2 most_s[2][4];  // of each 32 keys of a tile: the largest K scale, the largest V scale's size
   __shared__ unsigned scan_s[CK_THREADS / 32];
   __shared__ int abort_s, last_s;
   __shared__ float m_s[128], l_s[128];
@@ -487,15 +492,15 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           }
           store(w, sm + (s0 & 1 ? C::OFF_V : C::OFF_K) + st * C::BYTES);
           if (s0 & 1) {
-            scale_s[st * 256 + dt] = sk;
-            scale_s[st * 256 + 128 + dt] = sv;
+            scale_s[st * 384 + dt] = sk;
+            scale_s[st * 384 + 128 + dt] = sv;
+            scale_s[st * 384 + 256 + dt] = kvq_size(sv);
             // largest scales of 32 keys (bits order like the values; a NaN does not count)
             const uint32_t kb = __float_as_uint(sk) & 0x7fffffffu, vb = __float_as_uint(sv) & 0x7fffffffu;
             const uint32_t km = __reduce_max_sync(0xffffffffu, kb > 0x7f800000u ? 0u : kb);
             const uint32_t vm = __reduce_max_sync(0xffffffffu, vb > 0x7f800000u ? 0u : vb);
             if (lane == 0) {
-              skm_s[st][dw] = km;
-              svm_s[st][dw] = vm;
+              most_s[st][dw] = make_float2(__uint_as_float(km), kvq_size(__uint_as_float(vm)));
             }
           }
           __syncwarp();
@@ -672,8 +677,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       const int p_lo = x.len - x.n + x.row0 / a.G, p_hi = x.len - x.n + (x.row0 + x.rows - 1) / a.G;
       const int in_lo = a.window ? p_hi - a.window + 1 : 0, in_hi = min(p_lo + 1, x.len) - CK_KEYS, in_pre = x.pre - CK_KEYS;
       const int r_lo = a.window ? pos - a.window + 1 : 0, r_hi = min(pos, x.len - 1);  // sees r_lo .. r_hi and 0 .. pre - 1
+      // m: the largest score plus V scale's size when the reference last moved
       float m = -INFINITY, l = 0.f, ref = 0.f;
-      int ev = -100;
       const int J = x.alt ? nt : 2 * nt;
 #pragma unroll 1
       for (int j = t; j < J && !dead; j += 2) {
@@ -683,8 +688,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
         dead = !wait(&v_full[st], f >> 1) || !wait(&s_full[t], ns++);
         if (dead) break;
         ck_fence_after();
-        const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 256);
-        const float4* vsc = ksc + 32;
+        const float4* ksc = reinterpret_cast<const float4*>(scale_s + st * 384);
+        const float4 *vsc = ksc + 32, *size4 = ksc + 64;
         const bool inner = (j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre;
         // x of columns GC c .. GC c + GC - 1; where the common tile has its own
         // code this one is kept small
@@ -716,10 +721,11 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
         };
         // Does the reference hold? The common tile (no cap, no bias, nothing
         // masked) asks a bound first, the largest raw product of 32 keys times
-        // their largest K scale, which needs no key's own scale.
+        // their largest K scale, plus their largest V scale's size, which needs
+        // no key's own scales.
         const bool fast = PLAIN && inner;
-        const int en = max(ev, min(100, (int)(max(max(svm_s[st][0], svm_s[st][1]), max(svm_s[st][2], svm_s[st][3])) >> 23) - 126));
         float mx = m;
+        const float hold = m + CkLift<F32>::MARGIN;
         if (fast) {
           float z[2][32];
           ck_ld32(s_tm, z[0]);
@@ -737,12 +743,14 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
               top[0] = fmaxf(top[0], fmaxf(w[i], w[i + 1]));
               top[1] = fmaxf(top[1], fmaxf(w[i + 2], w[i + 3]));
             }
-            if (__any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) * (__uint_as_float(skm_s[st][c]) * rmul) <= m + CkLift<F32>::MARGIN))) {
+            const float2 most = most_s[st][c];
+            if (__any_sync(0xffffffffu, !(fmaf(fmaxf(top[0], top[1]), most.x * rmul, most.y) <= hold))) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float4 k4 = ksc[8 * c + i];
-                const float e0 = fmaxf(w[4 * i] * k4.x, w[4 * i + 1] * k4.y), e1 = fmaxf(w[4 * i + 2] * k4.z, w[4 * i + 3] * k4.w);
-                mx = fmaxf(mx, fmaxf(e0, e1) * rmul);
+                const float4 k4 = ksc[8 * c + i], z4 = size4[8 * c + i];
+                const float e0 = fmaxf(fmaf(w[4 * i] * rmul, k4.x, z4.x), fmaf(w[4 * i + 1] * rmul, k4.y, z4.y));
+                const float e1 = fmaxf(fmaf(w[4 * i + 2] * rmul, k4.z, z4.z), fmaf(w[4 * i + 3] * rmul, k4.w, z4.w));
+                mx = fmaxf(mx, fmaxf(e0, e1));
               }
             }
           }
@@ -752,16 +760,18 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             float z[GC];
             scores(c, z);
 #pragma unroll
-            for (int i = 0; i < GC; ++i) mx = fmaxf(mx, z[i]);
+            for (int i = 0; i < GC / 4; ++i) {
+              const float4 z4 = size4[GC / 4 * c + i];
+              mx = fmaxf(mx, fmaxf(fmaxf(z[4 * i] + z4.x, z[4 * i + 1] + z4.y), fmaxf(z[4 * i + 2] + z4.z, z[4 * i + 3] + z4.w)));
+            }
             if constexpr (GC == 32) ck_st32(s_tm + GC * c, z);  // tanh, bias and mask once only
           }
           if constexpr (GC == 32) ck_wait_st();
         }
-        if (__any_sync(0xffffffffu, mx > m + CkLift<F32>::MARGIN || en > ev)) {
-          const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT + (float)en;
+        if (__any_sync(0xffffffffu, mx > hold)) {
+          const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT;
           const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
           m = mx;
-          ev = en;
           ref = rn;
           l *= fac;
           if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)

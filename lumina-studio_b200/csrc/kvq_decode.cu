@@ -17,9 +17,11 @@
 // half's math, and no shared memory or barrier is in the loop. The scores are
 // transposed, S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, so that
 // 16 keys (or dims) fill the tensor pipe's 16 rows and the few query rows its
-// 8 columns. The scales stay outside the products (kvq_mma.cuh). The running
-// maximum moves only when a score passes it by 2^8 (p stays below 2^8), so
-// the steady state has no shuffles.
+// 8 columns. The scales stay outside the products (kvq_mma.cuh). A row's
+// reference is its own largest score times value scale (p times that scale
+// has to fit fp16, and a key that the row does not see, or hardly, takes
+// nothing from the others); it moves only when a key passes it by 2^8, so the
+// steady state has no shuffles.
 //
 // Measured: 64 sequences of up to 8192 tokens, 32 / 8 heads of 128, int8, fp16
 // rows: 87 us, 0.71 of the copy rate; 2 sequences of up to 131072, 32 / 4
@@ -369,12 +371,13 @@ kvq_decode_kernel(AttendArgs a) {
     float oz[FAST ? NR : 1][4];  // the zero points' product
 #pragma unroll
     for (int r = 0; r < (FAST ? NR : 1); ++r) oz[r][0] = oz[r][1] = oz[r][2] = oz[r][3] = 0.f;
-    float m[NR][2], l[NR][2], ms[NR][2];  // ms: m, 0 while nothing was seen
+    // m: the largest score plus V scale's size (kvq_size) when it last moved.
+    // p = 2^(x - ms), ms = m - 7 (0 while nothing was seen): times its V scale
+    // below 2^15, whatever the sizes of the V scales
+    float m[NR][2], l[NR][2], ms[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = ms[r][0] = ms[r][1] = 0.f;
-    int ev = -100;  // V scales are taken relative to 2^ev
     const float sign = FAST && (g & 1) ? -1.f : 1.f;  // odd keys' p (v_raw)
-    float vmul = sign * exp2i(7 + 100);
 
     // cells that start in [in_lo, in_hi] are seen by every row, as are those
     // that end within the prefix
@@ -484,11 +487,13 @@ kvq_decode_kernel(AttendArgs a) {
               if (!see) p[n][r][e] = -INFINITY;
             }
       }
-      // a score past the maximum by 2^8, or a V scale past 2^ev
+      // past the reference by 2^8? A bound first: the thread's largest score
+      // and largest V scale
       float svm = 0.f;
 #pragma unroll
       for (int n = 0; n < NK; ++n) svm = fmaxf(svm, fmaxf(fabsf(sv[n][0]), fabsf(sv[n][1])));
-      bool up = svm * fabsf(vmul) > 128.f;
+      svm = kvq_size(svm);
+      bool up = false;
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -496,15 +501,14 @@ kvq_decode_kernel(AttendArgs a) {
           float mx = fmaxf(p[0][r][c2], p[0][r][2 + c2]);
 #pragma unroll
           for (int n = 1; n < NK; ++n) mx = fmaxf(mx, fmaxf(p[n][r][c2], p[n][r][2 + c2]));
-          up |= mx > m[r][c2] + 8.f;
+          up |= mx + svm > m[r][c2] + 8.f;
         }
       if (__any_sync(0xffffffffu, up)) {
+        float size[NK][2];
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, d));
-        const int en = max(ev, min(100, (int)(__float_as_uint(svm) >> 23) - 126));
-        const float es = exp2i(max(-126, ev - en));
-        ev = en;
-        vmul = sign * exp2i(7 - en);
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) size[n][h] = kvq_size(sv[n][h]);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           float fac[2];
@@ -512,14 +516,13 @@ kvq_decode_kernel(AttendArgs a) {
           for (int c2 = 0; c2 < 2; ++c2) {
             float mx = m[r][c2];
 #pragma unroll
-            for (int n = 0; n < NK; ++n) mx = fmaxf(mx, fmaxf(p[n][r][c2], p[n][r][2 + c2]));
+            for (int n = 0; n < NK; ++n) mx = fmaxf(mx, fmaxf(p[n][r][c2] + size[n][0], p[n][r][2 + c2] + size[n][1]));
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            ms[r][c2] = mx == -INFINITY ? 0.f : mx;
-            fac[c2] = ex2(m[r][c2] - ms[r][c2]);
+            ms[r][c2] = mx == -INFINITY ? 0.f : mx - 7.f;
+            fac[c2] = mx == -INFINITY ? 1.f : ex2(m[r][c2] - mx);
             m[r][c2] = mx;
             l[r][c2] *= fac[c2];
-            fac[c2] *= es;
           }
 #pragma unroll
           for (int i = 0; i < NT / 2; ++i)
@@ -534,7 +537,7 @@ kvq_decode_kernel(AttendArgs a) {
       uint32_t pt[NK][NR][2], ptl[F32 ? NK : 1][F32 ? NR : 1][2];
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
-        const float vs[2] = {sv[n][0] * vmul, sv[n][1] * vmul};
+        const float vs[2] = {sv[n][0] * sign, sv[n][1] * sign};
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           float y[4];
@@ -628,7 +631,7 @@ kvq_decode_kernel(AttendArgs a) {
         float M = m_s[0][rr];
 #pragma unroll
         for (int w = 1; w < W; ++w) M = fmaxf(M, m_s[w][rr]);
-        const float f = ex2(m[r][c] - (M == -INFINITY ? 0.f : M)) * exp2i(ev - 7);
+        const float f = ex2(m[r][c] - (M == -INFINITY ? 0.f : M));
         float* dst = slab + (warp * R + rr) * C::LD + g * NT;
 #pragma unroll
         for (int i = 0; i < NT / 4; ++i)

@@ -55,6 +55,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
 
+// A V scale's size as attention's references count it: the e with |s| < 2^e,
+// -90 at least (a NaN too), so that 2^(15 - e) times any number of keys stays
+// within fp32. (Keys whose V scales are 2^126 apart may lose each other's
+// weights.)
+__device__ __forceinline__ float kvq_size(float s) {
+  const uint32_t b = __float_as_uint(s) & 0x7fffffffu;
+  return (float)(b > 0x7f800000u ? -90 : max(-90, (int)(b >> 23) - 126));
+}
+
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

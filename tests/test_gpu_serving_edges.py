@@ -110,3 +110,70 @@ def test_work_past_the_lines_of_tiles(sv, io, heads, rows):
     pool.attend(batch, torch.zeros_like(out), out=out)
     assert cuda.fault_status(0) == sv.FAULT_DATA
     assert (out == 77.0).all()
+
+
+ROWS = [5, 60, 80]  # the decode kernel; the chunk kernel with one and with two tiles of rows
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("bits,hd", [(8, 128), (4, 64)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("slope", [0.0, 0.01])
+def test_a_large_value_that_only_later_rows_see(sv, io, bits, hd, rows, window, slope):
+    """The last key's values are 2^40 times the others': the rows before the
+    last do not see it and are as exact as ever."""
+    import torch
+    rng = np.random.default_rng(31)
+    ln, heads, n_kv, page = 250, 4, 2, 16
+    k, v = rng.standard_normal((2, ln, n_kv, hd))
+    v[-1] *= 2.0 ** 40
+    pool, table = pool_of(rng, k, v, bits, page)
+    q = dev((2 * rng.standard_normal((rows, heads, hd))).astype(np.float32), getattr(torch, io))
+    got, want = attend_both(sv, pool, table, bits, hd, page, q, ln, np.full(heads, slope, np.float32) if slope else None, window)
+    check_attend(got[:-1], want[:-1], io)
+    if io == "float32":  # (an fp16 result of 2^40 is an infinity)
+        check_attend(got[-1:], want[-1:], io)
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("bits,hd", [(8, 128), (4, 64)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("at", [0, 30, 140])
+def test_a_large_value_of_vanishing_weight(sv, io, bits, hd, rows, at):
+    """A key that every row sees, with values 2^30 times the others' and a
+    weight below 2^-80: it adds nothing, and takes nothing from the others."""
+    import torch
+    rng = np.random.default_rng(32)
+    ln, heads, n_kv, page = 250, 4, 2, 16
+    base = 2 * rng.standard_normal((1, 1, hd))
+    k, v = rng.standard_normal((2, ln, n_kv, hd))
+    k[at] = -2 * base
+    v[at] *= 2.0 ** 30
+    pool, table = pool_of(rng, k, v, bits, page)
+    q = dev((base + 0.3 * rng.standard_normal((rows, heads, hd))).astype(np.float32), getattr(torch, io))
+    got, want = attend_both(sv, pool, table, bits, hd, page, q, ln)
+    check_attend(got, want, io)
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("rows", [1, *ROWS])
+def test_values_of_all_sizes(sv, io, rows):
+    """Values whose sizes spread from 2^-30 to 2^8 over the keys, some of
+    them zero rows."""
+    import torch
+    rng = np.random.default_rng(33)
+    ln, heads, n_kv, page, hd = 700, 4, 2, 16, 128
+    k, v = rng.standard_normal((2, ln, n_kv, hd))
+    v *= 2.0 ** rng.uniform(-30, 8, (ln, 1, 1))
+    pool, table = pool_of(rng, k, v, 8, page)
+    t = np.arange(0, ln, 7)
+    set_scales(pool, 8, hd, page, 1, table[0, t // page], t % page, 0.0)
+    q = dev((2 * rng.standard_normal((rows, heads, hd))).astype(np.float32), getattr(torch, io))
+    got, want = attend_both(sv, pool, table, 8, hd, page, q, ln)
+    check_attend(got, want, io)
+    # nothing but zero rows: zeros
+    t = np.arange(ln)
+    set_scales(pool, 8, hd, page, 1, table[0, t // page], t % page, 0.0)
+    got, _ = attend_both(sv, pool, table, 8, hd, page, q, ln)
+    assert (got == 0).all()
