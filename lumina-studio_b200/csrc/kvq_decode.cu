@@ -77,15 +77,13 @@ kvq_decode_kernel(AttendArgs a) {
   using C = DecCfg<HD, BITS, NR, F32>;
   using F = typename C::F;
   constexpr int KK = F::KK, NT = F::NT, W = C::W, R = C::R, NK = C::NK, CELL = C::CELL;
-  // fp16 rows spend no instructions on making numbers of the codes:
-  //  int8 K  integer products with q as two int8 planes, q = a (256 h + l)
-  //  int4 K  codes with their fp16 offset (1024 + ...), which a start value of
-  //          the accumulator takes off again
-  //  V       raw codes as fp16 subnormals, zero point by one more product
-  // (q at 2^-16 of its largest value and sums of the offsets' size cost 2^-14
-  // of a score at most, below the fp16 rounding of p). fp32 rows use exact
-  // signed codes and split q and p.
-  constexpr bool FAST = !F32, IK = FAST && BITS == 8, OFFSET = FAST && BITS == 4;
+  // fp16 rows spend next to no instructions on making numbers of the codes: K
+  // and V enter the products raw, as fp16 subnormals (KvqFrag), and the zero
+  // points come off again, K's as a start value of the accumulator, V's by one
+  // more product. q is exact (to 2^-35 of its largest value) and the sums are
+  // fp32 over terms of up to twice the codes' size, so a score is right to
+  // about 2^-22 of sum |q k|. fp32 rows use signed codes and split q and p.
+  constexpr bool FAST = !F32;
   // a chunk kernel of the same call may take the SMs that this one leaves
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint8_t sm[];
@@ -275,8 +273,8 @@ kvq_decode_kernel(AttendArgs a) {
   for (unsigned u = u0; u < u1; u += x.hi - x.lo) {
     segment(u, x);
     // this thread's rows: 8 o + g in the Q fragments, 8 o + 2 t + c in the scores
-    uint32_t qh[NR][KK][2], ql[F32 ? NR : 1][KK][2];  // IK: [step][plane h: 0, 1 | plane l: 0, 1] in the 2 KK / 2 words
-    float qmul[NR][2], off[OFFSET ? NR : 1][2], slope[PLAIN ? 1 : NR][2];
+    uint32_t qh[NR][KK][2], ql[F32 ? NR : 1][KK][2];
+    float qmul[NR][2], off[FAST ? NR : 1][2], slope[PLAIN ? 1 : NR][2];
     int pos[NR][2];
     const float scale = !PLAIN && a.cap > 0.f ? a.scale / a.cap : a.scale * KVQ_LOG2E;
 #pragma unroll
@@ -297,64 +295,38 @@ kvq_decode_kernel(AttendArgs a) {
         }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      float mul, of = 0.f;
-      if constexpr (IK) {
-        const float am = __uint_as_float(top), to = top ? 32639.f / am : 0.f;
-        mul = top < 0x7f800000u ? scale * (am / 32639.f) : __uint_as_float(0x7fffffffu);
+      // bring the row's largest value near 2^10: room for 16 q, and for what
+      // hi leaves to lo
+      const int ex = min(112, max(-112, (int)(top >> 23) - 127));
+      const float up = exp2i(10 - ex);
+      float mul = scale * exp2i(ex - 10), zero = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          uint32_t h = 0, l = 0;
+      for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = __float2int_rn(q[kk][e] * to), hi = (i + 128) >> 8;
-            h |= (uint32_t)(hi & 0xFF) << (8 * e);
-            l |= (uint32_t)((i - 256 * hi) & 0xFF) << (8 * e);
-          }
-          // step kk / 2 takes word kk as its half kk % 2
-          qh[o][(kk >> 1) * 2][kk & 1] = h;
-          qh[o][(kk >> 1) * 2 + 1][kk & 1] = l;
+        for (int e = 0; e < 4; ++e) q[kk][e] *= up;
+        if constexpr (F32) {
+          qh[o][kk][0] = split_h2(q[kk][0], q[kk][1], ql[o][kk][0]);
+          qh[o][kk][1] = split_h2(q[kk][2], q[kk][3], ql[o][kk][1]);
+        } else {  // (plain, complemented) pairs as k_raw gives them
+          constexpr int A = BITS == 8 ? 1 : 2, B = BITS == 8 ? 2 : 1;
+          constexpr float LOW = BITS == 8 ? 1.f : 16.f;  // int4: b1's codes come times 16
+          constexpr float Z0 = F::RAW_ZERO[0], Z1 = F::RAW_ZERO[1];
+          zero += Z0 * (q[kk][0] + q[kk][A]) - Z1 * (q[kk][B] + q[kk][3]);
+          qh[o][kk][0] = half2_bits(__floats2half2_rn(LOW * q[kk][0], -LOW * q[kk][B]));
+          qh[o][kk][1] = half2_bits(__floats2half2_rn(q[kk][A], -q[kk][3]));
         }
-      } else {
-        // bring the row's largest value near 2^10: room for 16 q, and for
-        // what hi leaves to lo
-        const int ex = min(112, max(-112, (int)(top >> 23) - 127));
-        const float up = exp2i(10 - ex);
-        float sum = 0.f, lo_sum = 0.f;
-        mul = scale * exp2i(ex - 10);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            q[kk][e] *= up;
-            sum += q[kk][e];
-            // e = 0, 1 are low nibbles (1024 + c), 2 and 3 high ones (1024 + 16 c)
-            if (OFFSET && e < 2) {
-              lo_sum += q[kk][e];
-              q[kk][e] *= 16.f;
-            }
-          }
-          if constexpr (F32) {
-            qh[o][kk][0] = split_h2(q[kk][0], q[kk][1], ql[o][kk][0]);
-            qh[o][kk][1] = split_h2(q[kk][2], q[kk][3], ql[o][kk][1]);
-          } else {
-            qh[o][kk][0] = half2_bits(__floats2half2_rn(q[kk][0], q[kk][1]));
-            qh[o][kk][1] = half2_bits(__floats2half2_rn(q[kk][2], q[kk][3]));
-          }
-        }
-        if constexpr (OFFSET) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          lo_sum += __shfl_xor_sync(0xffffffffu, lo_sum, 1);
-          lo_sum += __shfl_xor_sync(0xffffffffu, lo_sum, 2);
-          of = -(1024.f * (sum - lo_sum) + 16384.f * lo_sum + 120.f * sum);
-          mul *= 0.125f;
-        }
+      }
+      if constexpr (FAST) {
+        zero += __shfl_xor_sync(0xffffffffu, zero, 1);
+        zero += __shfl_xor_sync(0xffffffffu, zero, 2);
+        zero *= BITS == 8 ? -0x1p-24f : -0x1p-20f;
+        mul *= BITS == 8 ? 0x1p24f : 0x1p21f;
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int rr = 8 * o + 2 * t + c;
         qmul[o][c] = __shfl_sync(0xffffffffu, mul, (2 * t + c) * 4);
-        if constexpr (OFFSET) off[o][c] = __shfl_sync(0xffffffffu, of, (2 * t + c) * 4);
+        if constexpr (FAST) off[o][c] = __shfl_sync(0xffffffffu, zero, (2 * t + c) * 4);
         const int li = rr < x.n * a.G ? rr / a.G : 0;
         pos[o][c] = x.p0 + li;
         if constexpr (!PLAIN)
@@ -388,57 +360,26 @@ kvq_decode_kernel(AttendArgs a) {
       const unsigned held = have;
       const bool inner = held == (1u << NK) - 1 && ((j0 >= in_lo && j0 <= in_hi) || j0 <= in_pre);
       float p[NK][NR][4];  // [tile][row octet][key half * 2 + row c]
-      if constexpr (IK) {
-        // |sum h c| < 2^21: started at the bits of 1.5 * 2^23, the integer sum
-        // is the float 1.5 * 2^23 + sum
-        constexpr int MAGIC = 0x4B400000;
-        int dh[NK][NR][4], dl[NK][NR][4];
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
+      for (int n = 0; n < NK; ++n)
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dh[n][r][e] = dl[n][r][e] = MAGIC;
+          for (int e = 0; e < 4; ++e) p[n][r][e] = FAST ? off[FAST ? r : 0][e & 1] : 0.f;
+      static_for<KK>([&](auto kc) {
+        constexpr int kk = decltype(kc)::value;
 #pragma unroll
-        for (int kk = 0; kk < KK / 2; ++kk)
+        for (int n = 0; n < NK; ++n) {
+          uint32_t f[4];
+          F::template k_frag<kk, FAST>(kw[n][0], f[0], f[2]);
+          F::template k_frag<kk, FAST>(kw[n][1], f[1], f[3]);
 #pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            const uint32_t f[4] = {kw[n][0][2 * kk], kw[n][1][2 * kk], kw[n][0][2 * kk + 1], kw[n][1][2 * kk + 1]};
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              mma_16832_s8(dh[n][r], f, qh[r][2 * kk][0], qh[r][2 * kk][1]);
-              mma_16832_s8(dl[n][r], f, qh[r][2 * kk + 1][0], qh[r][2 * kk + 1][1]);
-            }
+          for (int r = 0; r < NR; ++r) {
+            if constexpr (F32) mma_16816(p[n][r], f, ql[r][kk][0], ql[r][kk][1]);
+            mma_16816(p[n][r], f, qh[r][kk][0], qh[r][kk][1]);
           }
-#pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              p[n][r][e] = fmaf(__int_as_float(dh[n][r][e]) - 12582912.f, 256.f, __int_as_float(dl[n][r][e]) - 12582912.f);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[n][r][e] = OFFSET ? off[OFFSET ? r : 0][e & 1] : 0.f;
-        static_for<KK>([&](auto kc) {
-          constexpr int kk = decltype(kc)::value;
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            uint32_t f[4];
-            F::template k_frag<kk, OFFSET>(kw[n][0], f[0], f[2]);
-            F::template k_frag<kk, OFFSET>(kw[n][1], f[1], f[3]);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              if constexpr (F32) mma_16816(p[n][r], f, ql[r][kk][0], ql[r][kk][1]);
-              mma_16816(p[n][r], f, qh[r][kk][0], qh[r][kk][1]);
-            }
-          }
-        });
-      }
+        }
+      });
       advance();
       load_k();
       if (!inner) {  // scales of keys that no row sees do not count

@@ -70,12 +70,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_16832_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 // (a, b) -> fp16 pair, and the fp16 pair of what it leaves
@@ -153,24 +147,28 @@ struct KvqFrag {
       w[0] = q.x; w[1] = q.y;
     }
   }
-  // fragment of step kk: k-indices e = 0, 1 in b0 and 2, 3 in b1. OFFSET
-  // leaves the fp16 numbers that hold the codes as they are, for callers that
-  // take the offset out of the product: 1152 + c (int8); 1024 + c in b0 and
-  // 1024 + 16 c in b1 (int4). Otherwise c (int8) or 2 c - 15 (int4).
-  template <int kk, bool OFFSET = false>
+  // fragment of step kk: k-indices e = 0, 1 in b0 and 2, 3 in b1, the codes'
+  // values c (int8) or 2 c - 15 (int4). RAW: unsigned codes at the bottom of
+  // an fp16 mantissa, that is the subnormal code * 2^-24 (exact on the tensor
+  // pipe), the second of each pair complemented: u = c + 128 and 255 - u
+  // (int8; e = 0, 2 in b0 and 1, 3 in b1); c and 15 - c, in b1 times 16 (int4).
+  // With q negated for the complemented ones, sum q (u - zero) = sum +-q u' -
+  // sum +-q w, w = RAW_ZERO of the place in the pair, and both sums stay small
+  // also where the q have a common offset.
+  template <int kk, bool RAW = false>
   __device__ static __forceinline__ void k_frag(const uint32_t (&w)[KW], uint32_t& b0, uint32_t& b1) {
-    if constexpr (BITS == 8 && OFFSET) {
-      const uint32_t f = w[kk] ^ 0x80808080u;
-      b0 = __byte_perm(f, 0x64646464u, 0x4140);
-      b1 = __byte_perm(f, 0x64646464u, 0x4342);
+    if constexpr (BITS == 8 && RAW) {
+      const uint32_t x = w[kk] ^ 0x7F7F8080u;
+      b0 = x & 0x00FF00FFu;
+      b1 = __byte_perm(x, 0u, 0x4341);  // bytes 1 and 3 (a shift and a mask: 93 us, 88 so, with 64 sequences of up to 8192)
     } else if constexpr (BITS == 8) {
       const uint32_t f = w[kk] ^ 0x80808080u;
       b0 = s8_pair<0x4140>(f);
       b1 = s8_pair<0x4342>(f);
-    } else if constexpr (OFFSET) {
+    } else if constexpr (RAW) {
       const uint32_t v = (kk & 1) ? w[kk >> 1] >> 8 : w[kk >> 1];
-      b0 = (v & 0x000F000Fu) | H_1024;
-      b1 = (v & 0x00F000F0u) | H_1024;
+      b0 = (v ^ 0x000F0000u) & 0x000F000Fu;
+      b1 = (v ^ 0x00F00000u) & 0x00F000F0u;
     } else {
       const uint32_t v = w[kk >> 1];
       b0 = u4_pair((kk & 1) ? v >> 4 : v << 4);
@@ -200,12 +198,8 @@ struct KvqFrag {
       return u4_pair((i & 3) == 0 ? x << 4 : x >> (4 * ((i & 3) - 1)));
     }
   }
-  // The same pairs as raw unsigned codes at the bottom of an fp16 mantissa,
-  // that is the subnormal code * 2^-24 (exact on the tensor pipe), the odd
-  // key's complemented: u = c + 128 and 255 - u (int8); c and 15 - c, for odd
-  // i times 16 (int4). With the odd keys' p negated, sum p (c - zero) =
-  // sum +-p u' - sum +-p w, w = RAW_ZERO of the key's parity, and the two
-  // sums stay small where sum p u would be 128 sum p.
+  // The same pairs raw (as in k_frag), the odd key's codes complemented and
+  // to be met by a negated p; for odd i int4 codes come times 16.
   static constexpr float RAW_ZERO[2] = {BITS == 8 ? 128.f : 7.5f, BITS == 8 ? 127.f : 7.5f};
   template <int i>
   __device__ static __forceinline__ uint32_t v_raw(uint32_t a, uint32_t b) {

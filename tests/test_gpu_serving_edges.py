@@ -177,3 +177,32 @@ def test_values_of_all_sizes(sv, io, rows):
     set_scales(pool, 8, hd, page, 1, table[0, t // page], t % page, 0.0)
     got, _ = attend_both(sv, pool, table, 8, hd, page, q, ln)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 80])
+@pytest.mark.parametrize("kind", ["one pair", "six pairs", "offset"])
+def test_outlier_dims(sv, io, bits, rows, kind):
+    """Outlier dims in q and K (scores of 100 to 1000 that differ little), and
+    a common offset of q. A score is an fp32 sum: at worst eight partial sums
+    that round at 2^-23 of sum |q k|, 2^-21 of it beyond the usual tolerance
+    (an error of a score is a relative error of its weight)."""
+    import torch
+    rng = np.random.default_rng(41)
+    ln, heads, n_kv, page, hd = 512, 4, 2, 16, 128
+    k, v = rng.standard_normal((2, ln, n_kv, hd))
+    q = 2 * rng.standard_normal((rows, heads, hd))
+    if kind == "offset":
+        q = 20 + 0.15 * q
+    else:
+        dims = rng.permutation(hd)[:2 if kind == "one pair" else 6]
+        size = 40 if kind == "one pair" else 100
+        q[..., dims] = size * (1 + 0.2 * rng.random((rows, heads, dims.size)))
+        k[..., dims] = 20 * (1 + 0.01 * rng.standard_normal((ln, n_kv, dims.size)))
+    pool, table = pool_of(rng, k, v, bits, page)
+    qd = dev(q.astype(np.float32), getattr(torch, io))
+    got, want = attend_both(sv, pool, table, bits, hd, page, qd, ln)
+    kk, _ = ref.rows_of(pool, table[0], ln, bits, hd, page)
+    dots = np.abs(qd.double().cpu().numpy()).reshape(rows, n_kv, -1, hd).transpose(1, 0, 2, 3).reshape(n_kv, -1, hd) @ np.abs(kk).transpose(1, 2, 0)
+    assert rel(got, want) < TOL[io] + 2.0 ** -21 * dots.max() * hd ** -0.5
