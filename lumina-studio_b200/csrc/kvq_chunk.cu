@@ -40,7 +40,8 @@
 // rows with cap, distance bias, window and prefix: 63 us.
 //
 // Waits are bounded: one that gives up sets bit 5 of the device fault word,
-// every role leaves its loop, and the CTA frees its tensor memory and exits.
+// every role leaves its loop, its rows stay unwritten (whoever joins their
+// parts), and the CTA frees its tensor memory and exits.
 #include <cfloat>
 #include <type_traits>
 
@@ -882,8 +883,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       if (x.alt) {
         // group 1 hands its state to group 0
         if (t == 1) {
-          m_s[row] = mine ? m : -INFINITY;
-          l_s[row] = mine ? l : 0.f;
+          l_s[row] = dead ? -1.f : mine ? l : 0.f;
           if (mine && have) {
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
@@ -921,7 +921,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       };
       if (!(x.alt && t == 1)) {
         float R = m == -INFINITY ? -INFINITY : ref, f2 = 0.f, L = l;
+        bool gone = dead;  // this row's state is not whole
         if (x.alt) {
+          gone |= l_s[row] < 0.f;
           const float r1 = m_s[row], M = fmaxf(R, r1);
           f1 = R == -INFINITY ? 0.f : ex2(R - M);
           f2 = r1 == -INFINITY ? 0.f : ex2(r1 - M);
@@ -951,7 +953,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
-          if (ok && !dead) {
+          if (ok && !gone) {
             if (split) {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -962,7 +964,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             }
           }
         }
-        if (split && ok) __stcg(reinterpret_cast<float2*>(my_part + (size_t)BM * HD) + (pr - x.row0), make_float2(R, L));
+        // (a sum below 0: the part is not there, and the row stays unwritten)
+        if (split && ok)
+          __stcg(reinterpret_cast<float2*>(my_part + (size_t)BM * HD) + (pr - x.row0), make_float2(R, gone ? -1.f : L));
       }
       ck_fence_before();
       pair_bar();  // Q tiles, merge buffer and O are free for the next segment
@@ -988,6 +992,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           auto weight = [](float2 rl, float M) { return rl.x == -INFINITY ? (rl.y == rl.y ? 0.f : rl.y) : ex2(rl.x - M); };
           if (tid < x.rows) {
             float M = -INFINITY, L = 0.f;
+            bool gone = false;
 #pragma unroll 4
             for (int p = 0; p < np; ++p) M = fmaxf(M, __ldcg(stat_of(p) + tid).x);
 #pragma unroll 4
@@ -995,9 +1000,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
               const float2 rl = __ldcg(stat_of(p) + tid);
               const float w = weight(rl, M);
               L += rl.y * w;
+              gone |= rl.y < 0.f;
               if (p < WT) wt[p * 256 + tid] = w;
             }
-            stat[tid] = make_float2(M, L);
+            stat[tid] = make_float2(M, gone ? -1.f : L);
           }
           pair_bar();
           constexpr int K = 2, GROUPS = HD / 32;
@@ -1031,7 +1037,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-              if (!there[k]) continue;
+              if (!there[k] || stat[r[k]].y < 0.f) continue;
               const float L = stat[r[k]].y, inv = L == 0.f ? 0.f : 1.0f / L;
               const bool none = L == 0.f;
               float o[8] = {y[k][0].x, y[k][0].y, y[k][0].z, y[k][0].w, y[k][1].x, y[k][1].y, y[k][1].z, y[k][1].w};

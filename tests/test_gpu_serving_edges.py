@@ -206,3 +206,36 @@ def test_outlier_dims(sv, io, bits, rows, kind):
     kk, _ = ref.rows_of(pool, table[0], ln, bits, hd, page)
     dots = np.abs(qd.double().cpu().numpy()).reshape(rows, n_kv, -1, hd).transpose(1, 0, 2, 3).reshape(n_kv, -1, hd) @ np.abs(kk).transpose(1, 2, 0)
     assert rel(got, want) < TOL[io] + 2.0 ** -21 * dots.max() * hd ** -0.5
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("hd,rows,lens", [
+    (128, [300], [2000]),            # parts of one task on many CTAs
+    (64, [50, 1, 40], [50, 90, 3000]),
+    (128, [1], [500]),               # for the decode kernel, which waits for nothing
+])
+def test_rows_of_a_wait_that_gave_up_stay_unwritten(sv, io, hd, rows, lens):
+    import torch
+    from lumina_b200 import cuda
+    rng = np.random.default_rng(51)
+    page, heads, n_kv = 16, 8, 2
+    table, n_pages, _ = layout(rng, lens, page)
+    pool = sv.KVPool(dev(random_pool(rng, n_pages, n_kv, 8, hd, page)), 8, hd, page)
+    q = dev(rng.standard_normal((sum(rows), heads, hd)).astype(np.float32), getattr(torch, io))
+    batch = batch_of(sv, rows, lens, table)
+    good = pool.attend(batch, q).clone()
+    out = torch.full_like(good, 77.0)
+    cuda.debug_wait_limit(0)
+    try:
+        pool.attend(batch, q, out=out)
+        torch.cuda.synchronize()
+        word = cuda.fault_status(0)
+    finally:
+        cuda.debug_wait_limit(-1)
+    at = 0
+    for n in rows:
+        few = n * heads // n_kv <= 32
+        assert torch.equal(out[at:at + n], good[at:at + n] if few else torch.full_like(good[at:at + n], 77.0))
+        at += n
+    assert word == (sv.FAULT_WAIT if max(rows) > 1 else 0)
+    assert torch.equal(pool.attend(batch, q, out=out), good)
