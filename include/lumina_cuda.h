@@ -130,13 +130,16 @@ int lumina_gemv_noalloc(const lumina_weight* w, const float* x_dev, int batch, i
  * peers (the decode GEMVs, the tcgen05 multi-row projection, the
  * tensor-parallel exchange) bound every wait; one that gives up ORs a bit
  * into a per-device fault word (1: gemv_fused, 2: gemv_tc, 4: peer exchange,
- * 8: gemm_tc05, 16: gemv_tcb, 32: lumina_kvq_attend) and returns, leaving its outputs unwritten. Every
+ * 8: gemm_tc05, 16: gemv_tcb) and returns, leaving its outputs unwritten. Every
  * synchronous entry (lumina_gemv_host, lumina_forward, lumina_layer_forward,
  * lumina_decode_step, lumina_decode_greedy, lumina_profile_gemv) clears the
  * word as it starts and returns LUMINA_E_CUDA ("a device wait timed out")
- * when it is set at the end. lumina_gemv, lumina_gemm_rows and
- * lumina_gemv_noalloc are asynchronous: after synchronizing their stream, the caller reads (and with
- * `clear`, resets) the word here. The tops-style reference reported no
+ * when it is set at the end. The batched serving calls (lumina_kvq_*) report
+ * apart, in a word of their own (32: a wait of lumina_kvq_attend, 64: batch
+ * data out of range), which those entries neither read nor clear.
+ * lumina_gemv, lumina_gemm_rows, lumina_gemv_noalloc and lumina_kvq_* are
+ * asynchronous: after synchronizing their stream, the caller reads (and with
+ * `clear`, resets) both words, ORed, here. The tops-style reference reported no
  * errors at all (tops_int8.c: void returns); the dict convention of
  * tops.py:296-314 carries this one to Python callers. */
 int lumina_fault_status(int device, int* word_host, int clear);

@@ -57,7 +57,7 @@ int kvq_view(const lumina_kvq_pool* p, const lumina_kvq_batch* b, const char* wh
   v->n_seq = b->n_seq;
   v->n_rows = b->n_rows;
   v->max_rows = b->max_rows;
-  v->fault = fault_flag_ptr();
+  v->fault = serving_fault_ptr();
   if (!v->fault) {
     set_error("%s: fault word unavailable on device %d", what, p->device);
     return LUMINA_E_CUDA;

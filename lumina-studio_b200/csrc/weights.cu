@@ -158,11 +158,14 @@ static void linspace_levels(int bits, double* out) {
 
 __constant__ double c_levels[4][16];
 
-// The device fault word: a bounded wait gave up in gemv_fused_kernel (bit
-// 0), gemv_tc_kernel (bit 1), the tensor-parallel peer exchange (bit 2) or
-// gemm_tc05_kernel (bit 3). Kernels only ever OR bits in; the host reads and
-// clears it (lumina_fault_status, and every synchronous entry).
-__device__ int g_fault_flag;
+// The device fault words. The first: a bounded wait gave up in
+// gemv_fused_kernel (bit 0), gemv_tc_kernel (bit 1), the tensor-parallel peer
+// exchange (bit 2), gemm_tc05_kernel (bit 3) or gemv_tcb_kernel (bit 4). Every
+// synchronous entry reads and clears it, and kernels only ever OR bits in. The
+// second is the batched serving calls' (bits 5 and 6), which may run beside
+// such an entry: neither fails nor clears the other. lumina_fault_status reads
+// and clears both.
+__device__ int g_fault_flag[2];
 
 int* fault_flag_ptr() {
   static std::mutex mu;
@@ -182,6 +185,11 @@ int* fault_flag_ptr() {
     p[dev] = static_cast<int*>(a);
   }
   return p[dev];
+}
+
+int* serving_fault_ptr() {
+  int* p = fault_flag_ptr();
+  return p ? p + 1 : nullptr;
 }
 
 int read_fault_flag(int* out) {
@@ -205,10 +213,9 @@ int clear_fault_async(cudaStream_t s) {
 }
 
 int fault_error(const char* what, int word) {
-  set_error("%s: a device wait timed out (fault word %#x:%s%s%s%s%s%s%s)", what, word,
+  set_error("%s: a device wait timed out (fault word %#x:%s%s%s%s%s)", what, word,
             (word & 1) ? " gemv_fused_kernel" : "", (word & 2) ? " gemv_tc_kernel" : "",
-            (word & 4) ? " peer exchange" : "", (word & 8) ? " gemm_tc05_kernel" : "", (word & 16) ? " gemv_tcb_kernel" : "",
-            (word & 32) ? " lumina_kvq_attend" : "", (word & 64) ? " lumina_kvq batch out of range" : "");
+            (word & 4) ? " peer exchange" : "", (word & 8) ? " gemm_tc05_kernel" : "", (word & 16) ? " gemv_tcb_kernel" : "");
   return LUMINA_E_CUDA;
 }
 
@@ -583,8 +590,10 @@ int lumina_fault_status(int device, int* word, int clear) {
     return LUMINA_E_CUDA;
   }
   LUMINA_CUDA_TRY(cudaDeviceSynchronize());
-  LUMINA_CUDA_TRY(cudaMemcpy(word, p, sizeof(int), cudaMemcpyDeviceToHost));
-  if (clear && *word) LUMINA_CUDA_TRY(cudaMemset(p, 0, sizeof(int)));
+  int words[2] = {0, 0};
+  LUMINA_CUDA_TRY(cudaMemcpy(words, p, sizeof(words), cudaMemcpyDeviceToHost));
+  *word = words[0] | words[1];
+  if (clear && *word) LUMINA_CUDA_TRY(cudaMemset(p, 0, sizeof(words)));
   return LUMINA_OK;
 }
 

@@ -262,6 +262,8 @@ void actq_carve(void* base, int batch, int nblk_pad, ActQ* out);
 // Device-side error word: bounded waits that give up set a bit here.
 int read_fault_flag(int* out);
 int* fault_flag_ptr();
+// the batched serving calls' own word
+int* serving_fault_ptr();
 // stream-ordered clear of the current device's fault word
 int clear_fault_async(cudaStream_t s);
 // LUMINA_E_CUDA with the text of a set fault word

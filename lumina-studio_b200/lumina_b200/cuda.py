@@ -211,8 +211,9 @@ def ptr(arr: np.ndarray, ctype):
 
 
 def fault_status(device: int = 0, clear: bool = True) -> int:
-    """The device's fault word after its queued work finished (non-zero: a
-    bounded wait inside an asynchronous GEMV gave up; see lumina_gemv)."""
+    """The device's fault words, ORed, after its queued work finished (1 to
+    16: a bounded wait inside an asynchronous GEMV gave up, see lumina_gemv;
+    32 and 64: the batched serving calls, see serving)."""
     lib = bound_lib()
     w = ctypes.c_int(0)
     check(lib.lumina_fault_status(int(device), ctypes.byref(w), 1 if clear else 0), lib)

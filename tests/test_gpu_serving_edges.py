@@ -239,3 +239,39 @@ def test_rows_of_a_wait_that_gave_up_stay_unwritten(sv, io, hd, rows, lens):
         at += n
     assert word == (sv.FAULT_WAIT if max(rows) > 1 else 0)
     assert torch.equal(pool.attend(batch, q, out=out), good)
+
+
+def test_serving_and_the_single_sequence_model_report_apart(sv, tiny_file):
+    """Bad batch data does not fail a step of the single-sequence model, and
+    the step does not clear what the batch reported; nor the reverse."""
+    import torch
+    from lumina_b200 import cuda, synthetic
+    from lumina_b200.cuda import LuminaError
+    from lumina_b200.engine import CudaChatModel
+    pool = sv.KVPool.empty(2, 1, 64, 8, 16)
+    pool.data.zero_()
+    bad = batch_of(sv, [1], [3], np.array([[9]], np.int32))  # page 9 of 2
+    q = torch.zeros(1, 1, 64, device="cuda")
+    m = CudaChatModel.from_lumina(tiny_file, synthetic.hf_cfg(synthetic.TINY), None, theta=synthetic.TINY["rope_theta"],
+                                  max_seq=64, max_rows=16)
+    try:
+        m.forward([1, 2, 3], 0)
+        side = torch.cuda.Stream()
+        for _ in range(20):
+            with torch.cuda.stream(side):
+                for _ in range(10):
+                    pool.attend(bad, q)
+            m.decode_step(4)
+            m.kv_truncate(3)
+        m.decode_greedy(4, 3)
+        assert cuda.fault_status(0, clear=False) == sv.FAULT_DATA
+        cuda.debug_wait_limit(0)
+        try:
+            with pytest.raises(LuminaError, match="timed out"):
+                m.forward([1, 2, 3], 0)
+        finally:
+            cuda.debug_wait_limit(-1)
+        assert cuda.fault_status(0) == sv.FAULT_DATA
+        assert cuda.fault_status(0) == 0
+    finally:
+        m.close()
