@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
               for (int e = 0; e < 4; ++e) {
                 const float y = ex2(z[4 * i + e] - ref);
                 l += y;
-                p[e] = y == 0.f ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
+                p[e] = z[4 * i + e] == -INFINITY ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
               }
               if constexpr (F32) {
                 ph[2 * i] = split_h2(p[0], p[1], pl[2 * i]);
@@ -938,15 +938,13 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           float o[32];
           ck_get32(o_tm + 32 * c, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = f1 == 0.f && L == L ? 0.f : o[i] * f1;
+          for (int i = 0; i < 32; ++i) o[i] *= f1;
           if (other) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float4 z = *at(row, 8 * c + i);
-              if (f2 != 0.f || L != L) {
-                o[4 * i] = fmaf(z.x, f2, o[4 * i]); o[4 * i + 1] = fmaf(z.y, f2, o[4 * i + 1]);
-                o[4 * i + 2] = fmaf(z.z, f2, o[4 * i + 2]); o[4 * i + 3] = fmaf(z.w, f2, o[4 * i + 3]);
-              }
+              o[4 * i] = fmaf(z.x, f2, o[4 * i]); o[4 * i + 1] = fmaf(z.y, f2, o[4 * i + 1]);
+              o[4 * i + 2] = fmaf(z.z, f2, o[4 * i + 2]); o[4 * i + 3] = fmaf(z.w, f2, o[4 * i + 3]);
             }
           }
           if (L == 0.f) {

@@ -481,16 +481,12 @@ kvq_decode_kernel(AttendArgs a) {
         const float vs[2] = {sv[n][0] * sign, sv[n][1] * sign};
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          float y[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            y[e] = ex2(p[n][r][e] - ms[r][e & 1]);
-            l[r][e & 1] += y[e];
-            p[n][r][e] = y[e] * vs[e >> 1];
-          }
-          if (!inner) {  // a masked key counts for nothing, whatever its scale holds
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[n][r][e] = y[e] == 0.f ? 0.f : p[n][r][e];
+            const float x = p[n][r][e], y = ex2(x - ms[r][e & 1]);
+            l[r][e & 1] += y;
+            // a masked key counts for nothing, whatever its scale holds
+            p[n][r][e] = !inner && x == -INFINITY ? 0.f : y * vs[e >> 1];
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {

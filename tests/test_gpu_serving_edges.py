@@ -275,3 +275,27 @@ def test_serving_and_the_single_sequence_model_report_apart(sv, tiny_file):
         assert cuda.fault_status(0) == 0
     finally:
         m.close()
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("rows", [1, *ROWS])
+@pytest.mark.parametrize("why", ["score", "distance"])
+@pytest.mark.parametrize("at", [3, 130, 240])
+def test_nan_values_behind_a_vanishing_weight(sv, io, rows, why, at):
+    """What sees a NaN row becomes NaN, also where the key's weight is too
+    small for a float; the other KV head does not."""
+    import torch
+    rng = np.random.default_rng(71)
+    ln, heads, n_kv, page, hd = 330, 4, 2, 16, 128
+    base = 4 * rng.standard_normal((1, 1, hd))
+    k, v = rng.standard_normal((2, ln, n_kv, hd))
+    if why == "score":
+        k[at] = -8 * base
+    pool, table = pool_of(rng, k, v, 8, page)
+    scales = np.array([np.nan, 1.0], np.float32)
+    set_scales(pool, 8, hd, page, 1, table[0, at // page], at % page, scales)
+    q = dev((base + 0.3 * rng.standard_normal((rows, heads, hd))).astype(np.float32), getattr(torch, io))
+    slopes = np.full(heads, 8.0, np.float32) if why == "distance" else None
+    got, want = attend_both(sv, pool, table, 8, hd, page, q, ln, slopes)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.isnan(want[at - (ln - rows) if at >= ln - rows else 0:, :2]).all() and not np.isnan(want[:, 2:]).any()
