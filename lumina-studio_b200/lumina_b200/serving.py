@@ -119,9 +119,19 @@ class SeqBatch:
 _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
 
+def _capturing(device: int) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if device == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def attend_workspace(device: int = 0) -> torch.Tensor:
-    """A zeroed workspace for ``KVPool.attend`` (one per stream that may run
-    it at the same time as another)."""
+    """A zeroed workspace for ``KVPool.attend``: one for each stream and each
+    captured graph whose calls may run at the same time as another's. Make it
+    outside any capture (the zeros have to be there before the first replay)
+    and keep it as long as the graph."""
     n = _SZ()
     check(_lib(device).lumina_kvq_workspace_bytes(device, ctypes.byref(n)))
     return torch.zeros(n.value, dtype=torch.uint8, device="cuda:%d" % device)
@@ -219,7 +229,9 @@ class KVPool:
         sqrt(head_dim); ``softcap`` c > 0 turns scores into c tanh(x / c);
         ``slopes`` (heads, float32) subtract slope * |p - j|. A row that sees
         nothing gives zeros. ``workspace``: ``attend_workspace(device)``, by
-        default one that this module keeps per stream."""
+        default one of about 50 MB that this module makes for each stream at its
+        first call and keeps. While a graph is captured there is no default:
+        a graph's calls need a workspace that is theirs at every replay."""
         b, hd, dev, n = self._batch(batch), self.head_dim, self.device, batch.n_rows
         dt, ty = q.dtype, self._type(q, "q")
         width = q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2]
@@ -231,6 +243,8 @@ class KVPool:
         ldo = _rows(out, dt, dev, n, width, "out")
         stream = _stream(dev)
         if workspace is None:
+            if _capturing(dev):
+                _bad("attend: a captured call needs a workspace of its own (attend_workspace, made outside the capture)")
             workspace = _WORKSPACES.get((dev, stream))
             if workspace is None:
                 workspace = _WORKSPACES[(dev, stream)] = attend_workspace(dev)

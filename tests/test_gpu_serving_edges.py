@@ -299,3 +299,39 @@ def test_nan_values_behind_a_vanishing_weight(sv, io, rows, why, at):
     got, want = attend_both(sv, pool, table, 8, hd, page, q, ln, slopes)
     assert np.array_equal(np.isnan(got), np.isnan(want))
     assert np.isnan(want[at - (ln - rows) if at >= ln - rows else 0:, :2]).all() and not np.isnan(want[:, 2:]).any()
+
+
+def test_capture_needs_a_workspace_of_its_own(sv):
+    """A capture without a workspace is refused, whether or not the stream
+    has a default one; two graphs with their own replay in either order."""
+    import torch
+    from lumina_b200.cuda import LuminaError
+    rng = np.random.default_rng(61)
+    hd, page, heads, n_kv, lens = 128, 16, 8, 2, [3000, 2500]
+    table, n_pages, _ = layout(rng, lens, page)
+    pool = sv.KVPool(dev(random_pool(rng, n_pages, n_kv, 8, hd, page)), 8, hd, page)
+    batch = batch_of(sv, [1, 1], lens, table)
+    q = [dev(rng.standard_normal((2, heads, hd)).astype(np.float32)) for _ in range(2)]
+    want = [pool.attend(batch, x).clone() for x in q]
+    out = [torch.empty_like(x) for x in q]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        pool.attend(batch, q[0])
+    torch.cuda.synchronize()
+    for stream in (None, side):
+        with pytest.raises(LuminaError, match="workspace"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+                pool.attend(batch, q[0], out=out[0])
+    ws = [sv.attend_workspace(0) for _ in range(2)]
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            pool.attend(batch, q[i], out=out[i], workspace=ws[i])
+    for order in ((1, 0), (0, 1)):
+        for x in out:
+            x.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for x, w in zip(out, want))
