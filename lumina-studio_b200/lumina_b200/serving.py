@@ -248,10 +248,13 @@ class KVPool:
             workspace = _WORKSPACES.get((dev, stream))
             if workspace is None:
                 workspace = _WORKSPACES[(dev, stream)] = attend_workspace(dev)
+            ws = workspace.data_ptr()
+        else:
+            ws = _vec(workspace, torch.uint8, dev, "workspace")
         a = _Attend(q.data_ptr(), out.data_ptr(), ldq, ldo, ty, width // hd, scale, softcap,
                     None if slopes is None else _vec(slopes, torch.float32, dev, "slopes", width // hd),
                     None if prefix is None else _vec(prefix, torch.int32, dev, "prefix", batch.n_seq), window,
-                    workspace.data_ptr(), workspace.numel())
+                    ws, workspace.numel())
         check(self.lib.lumina_kvq_attend(ctypes.byref(self.c), b, ctypes.byref(a), stream), self.lib)
         return out
 

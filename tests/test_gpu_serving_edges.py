@@ -335,3 +335,20 @@ def test_capture_needs_a_workspace_of_its_own(sv):
             graphs[i].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, w) for x, w in zip(out, want))
+
+
+@pytest.mark.parametrize("make", [
+    lambda n: np.zeros(n, np.uint8),
+    lambda n: dev(np.zeros(n // 4, np.float32)),
+    lambda n: dev(np.zeros(2 * n, np.uint8))[::2],
+    lambda n: dev(np.zeros(n - 1, np.uint8)),
+    lambda n: dev(np.zeros(n + 1, np.uint8))[1:],
+], ids=["host memory", "other type", "strided", "short", "misaligned"])
+def test_workspaces_that_are_refused(sv, make):
+    import torch
+    from lumina_b200.cuda import LuminaError
+    ws = make(sv.attend_workspace(0).numel())
+    pool = sv.KVPool.empty(4, 2, 64, 8, 16)
+    batch = batch_of(sv, [2], [20], np.zeros((1, 2), np.int32))
+    with pytest.raises(LuminaError):
+        pool.attend(batch, torch.zeros(2, 4, 64, device="cuda"), workspace=torch.from_numpy(ws) if isinstance(ws, np.ndarray) else ws)
