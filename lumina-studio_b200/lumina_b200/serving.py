@@ -82,7 +82,7 @@ def _vec(t, dtype, device, name, n=None):
 def _rows(t, dtype, device, n, width, name):
     """Rows of ``width`` contiguous elements: (n, width) or (n, heads, dim)
     with the heads side by side. Returns the row stride."""
-    if t.dtype is not dtype or t.get_device() != device or t.shape[0] != n:
+    if t.dim() < 2 or t.dtype is not dtype or t.get_device() != device or t.shape[0] != n:
         _bad("%s: %s%s on %s, %d rows of %s on cuda:%d are needed" % (name, t.dtype, tuple(t.shape), t.device, n, dtype, device))
     st = t.stride()
     if t.dim() == 2:
@@ -178,6 +178,12 @@ class KVPool:
             _bad("%s: %s, float32 or float16 is needed" % (name, t.dtype))
         return code
 
+    def _width(self, q):
+        width = q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2] if q.dim() == 3 else 0
+        if width == 0 or width % self.head_dim:
+            _bad("q: shape %s, rows of a multiple of head dim %d are needed" % (tuple(q.shape), self.head_dim))
+        return width
+
     def append(self, batch: SeqBatch, q, k, v, cos, sin, q_norm=None, k_norm=None, eps: float = 1e-6, out=None):
         """Write the batch's new rows: q (n_rows, heads, head_dim), k and v
         (n_rows, n_kv, head_dim) -- or the same as 2-D column ranges of one
@@ -186,9 +192,7 @@ class KVPool:
         ``cos`` / ``sin`` (n_pos, head_dim / 2). Returns the rotated queries."""
         b, hd, dev, n = self._batch(batch), self.head_dim, self.device, batch.n_rows
         dt, ty = q.dtype, self._type(q, "q")
-        width = q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2]
-        if width % hd:
-            _bad("q: rows of %d, a multiple of head dim %d is needed" % (width, hd))
+        width = self._width(q)
         ldq = _rows(q, dt, dev, n, width, "q")
         ldk = _rows(k, dt, dev, n, self.n_kv * hd, "k")
         ldv = _rows(v, dt, dev, n, self.n_kv * hd, "v")
@@ -234,9 +238,7 @@ class KVPool:
         a graph's calls need a workspace that is theirs at every replay."""
         b, hd, dev, n = self._batch(batch), self.head_dim, self.device, batch.n_rows
         dt, ty = q.dtype, self._type(q, "q")
-        width = q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2]
-        if width % hd:
-            _bad("q: rows of %d, a multiple of head dim %d is needed" % (width, hd))
+        width = self._width(q)
         ldq = _rows(q, dt, dev, n, width, "q")
         if out is None:
             out = torch.empty((n, width // hd, hd), dtype=dt, device=q.device)
@@ -299,10 +301,10 @@ def adjust_logits(logits, history=None, repeat=None, frequency=None, presence=No
         a.bias_val_dev = _vec(bias[2], torch.float32, dev, "bias values", bias[1].numel())
         a.bias_len = bias[1].numel()
     if mask is not None:
-        a.mask_dev = _vec(mask, torch.int32, dev, "mask")
-        a.mask_ld = mask.shape[1]
         if mask.dim() != 2 or mask.shape[0] != R:
             _bad("mask: %s, (%d, words) is needed" % (tuple(mask.shape), R))
+        a.mask_dev = _vec(mask, torch.int32, dev, "mask")
+        a.mask_ld = mask.shape[1]
     if argmax is not False:
         a.argmax_dev = _vec(argmax, torch.int32, dev, "argmax", R)
     check(lib.lumina_logits_adjust(ctypes.byref(a), _stream(dev)), lib)

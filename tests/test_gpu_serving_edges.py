@@ -301,6 +301,7 @@ def test_nan_values_behind_a_vanishing_weight(sv, io, rows, why, at):
     assert np.isnan(want[at - (ln - rows) if at >= ln - rows else 0:, :2]).all() and not np.isnan(want[:, 2:]).any()
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_capture_needs_a_workspace_of_its_own(sv):
     """A capture without a workspace is refused, whether or not the stream
     has a default one; two graphs with their own replay in either order."""
@@ -352,3 +353,24 @@ def test_workspaces_that_are_refused(sv, make):
     batch = batch_of(sv, [2], [20], np.zeros((1, 2), np.int32))
     with pytest.raises(LuminaError):
         pool.attend(batch, torch.zeros(2, 4, 64, device="cuda"), workspace=torch.from_numpy(ws) if isinstance(ws, np.ndarray) else ws)
+
+
+def test_tensors_of_too_few_dims_are_refused(sv):
+    import torch
+    from lumina_b200.cuda import LuminaError
+    pool = sv.KVPool.empty(2, 1, 64, 8, 16)
+    batch = batch_of(sv, [1], [1], np.zeros((1, 1), np.int32))
+    q, kv, cs = torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 64, device="cuda"), torch.zeros(4, 32, device="cuda")
+    logits = torch.zeros(2, 64, device="cuda")
+    for call in (lambda: pool.attend(batch, q.flatten()),
+                 lambda: pool.attend(batch, q[0, 0, 0]),
+                 lambda: pool.attend(batch, q, out=q.flatten()),
+                 lambda: pool.append(batch, q.flatten(), kv, kv, cs, cs),
+                 lambda: pool.append(batch, q, kv.flatten(), kv, cs, cs),
+                 lambda: pool.append(batch, q, kv[0, 0], kv, cs, cs),
+                 lambda: pool.append(batch, q[:, :0], kv, kv, cs, cs),
+                 lambda: pool.read(batch, out=(kv.flatten(), kv)),
+                 lambda: sv.adjust_logits(logits, out=logits.flatten()),
+                 lambda: sv.adjust_logits(logits, mask=torch.zeros(4, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(LuminaError):
+            call()
