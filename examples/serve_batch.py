@@ -152,6 +152,9 @@ class BatchModel:
         """Run every request to its end: a step holds one row of each request
         that generates and up to ``chunk`` rows of one prompt. Returns the
         generated tokens of each."""
+        for r in requests:
+            if not 0 < len(r.prompt) <= self.max_seq:
+                raise ValueError("a prompt of %d tokens, 1 to %d are served" % (len(r.prompt), self.max_seq))
         live = list(requests)
         while live:
             rows, tokens = [], []

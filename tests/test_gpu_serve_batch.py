@@ -83,3 +83,14 @@ def test_out_of_pages(tiny_file):
     model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], n_pages=2)
     with pytest.raises(RuntimeError, match="out of pages"):
         model.serve([sb.Request([1] * 40)])
+
+
+def test_prompts_past_the_tables_are_refused(tiny_file):
+    import serve_batch as sb
+    model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], max_seq=64)
+    for n in (0, 65):
+        with pytest.raises(ValueError, match="prompt"):
+            model.serve([sb.Request([1] * 5), sb.Request([1] * n)])
+    out = model.serve([sb.Request([1] * 64, max_tokens=3), sb.Request([1] * 63, max_tokens=3)])
+    assert [len(o) for o in out] == [1, 2]  # the tables end there
+    assert len(model.free) == 256
