@@ -151,11 +151,22 @@ class BatchModel:
     def serve(self, requests, chunk=64):
         """Run every request to its end: a step holds one row of each request
         that generates and up to ``chunk`` rows of one prompt. Returns the
-        generated tokens of each."""
+        generated tokens of each; an error leaves the requests cut off."""
         for r in requests:
             if not 0 < len(r.prompt) <= self.max_seq:
                 raise ValueError("a prompt of %d tokens, 1 to %d are served" % (len(r.prompt), self.max_seq))
-        live = list(requests)
+        try:
+            self._serve(list(requests), chunk)
+        finally:  # the pages of requests that an error cut off
+            for r in requests:
+                self._release(r)
+        return [r.out for r in requests]
+
+    def _release(self, r):
+        self.free += r.pages
+        r.pages = []
+
+    def _serve(self, live, chunk):
         while live:
             rows, tokens = [], []
             budget, batch_reqs = chunk, []
@@ -186,10 +197,8 @@ class BatchModel:
             for r, t in zip(giving, self.pick(logits, giving)):
                 r.out.append(t)
                 if t in r.stop or len(r.out) >= r.max_tokens or len(r.prompt) + len(r.out) > self.max_seq:
-                    self.free += r.pages
-                    r.pages = []
+                    self._release(r)
                     live.remove(r)
-        return [r.out for r in requests]
 
 
 def main():

@@ -94,3 +94,12 @@ def test_prompts_past_the_tables_are_refused(tiny_file):
     out = model.serve([sb.Request([1] * 64, max_tokens=3), sb.Request([1] * 63, max_tokens=3)])
     assert [len(o) for o in out] == [1, 2]  # the tables end there
     assert len(model.free) == 256
+
+
+def test_pages_return_when_the_pool_runs_dry(tiny_file):
+    import serve_batch as sb
+    model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], n_pages=4)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        model.serve([sb.Request([1] * 20), sb.Request([1] * 50)])
+    assert sorted(model.free) == list(range(4))
+    assert len(model.serve([sb.Request([1] * 20, max_tokens=2)])[0]) == 2
