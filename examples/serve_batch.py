@@ -116,7 +116,7 @@ class BatchModel:
             self._project(w["down"], torch.nn.functional.silu(ff[0]) * ff[1], y)
             x += y
         # no norm before the head, as in the single-sequence model
-        return x[torch.tensor(last, device=self.device)] @ self.head.float().T
+        return x[torch.tensor(last, dtype=torch.long, device=self.device)] @ self.head.float().T
 
     def grow(self, r, tokens):
         while len(r.pages) * self.page_size < tokens:

@@ -103,3 +103,12 @@ def test_pages_return_when_the_pool_runs_dry(tiny_file):
         model.serve([sb.Request([1] * 20), sb.Request([1] * 50)])
     assert sorted(model.free) == list(range(4))
     assert len(model.serve([sb.Request([1] * 20, max_tokens=2)])[0]) == 2
+
+
+def test_steps_that_give_no_token(tiny_file):
+    """A prompt of several chunks with nothing beside it."""
+    import serve_batch as sb
+    model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], n_pages=16)
+    prompt = np.random.default_rng(5).integers(0, CFG["vocab_size"], 100).tolist()
+    whole = model.serve([sb.Request(prompt, max_tokens=1)], chunk=128)
+    assert model.serve([sb.Request(prompt, max_tokens=1)], chunk=30) == whole
