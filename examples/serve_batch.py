@@ -24,7 +24,7 @@ import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "lumina-studio_b200"))
 
-from lumina_b200 import serving  # noqa: E402
+from lumina_b200 import cuda, serving  # noqa: E402
 from lumina_b200.cuda import LuminaError  # noqa: E402
 from lumina_b200.engine import rope_tables  # noqa: E402
 from lumina_b200.loader import LuminaFile, upload_record  # noqa: E402
@@ -191,10 +191,12 @@ class BatchModel:
                 n_rows=int(start[-1]), max_rows=max(rows))
             gives = [i for i, r in enumerate(batch_reqs) if not r.waiting()]
             logits = self.step(tokens, batch, [int(start[i + 1]) - 1 for i in gives])
-            if not gives:
-                continue
             giving = [batch_reqs[i] for i in gives]
-            for r, t in zip(giving, self.pick(logits, giving)):
+            picked = self.pick(logits, giving) if giving else []
+            word = cuda.fault_status(self.device.index)  # a wait that gave up, a page or length out of range
+            if word:
+                raise RuntimeError("the step's rows are not whole: fault word %d" % word)
+            for r, t in zip(giving, picked):
                 r.out.append(t)
                 if t in r.stop or len(r.out) >= r.max_tokens or len(r.prompt) + len(r.out) > self.max_seq:
                     self._release(r)

@@ -112,3 +112,16 @@ def test_steps_that_give_no_token(tiny_file):
     prompt = np.random.default_rng(5).integers(0, CFG["vocab_size"], 100).tolist()
     whole = model.serve([sb.Request(prompt, max_tokens=1)], chunk=128)
     assert model.serve([sb.Request(prompt, max_tokens=1)], chunk=30) == whole
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+def test_a_step_with_a_fault_gives_no_tokens(tiny_file, rows):
+    """A page number out of range, made on the host: the kernels report it."""
+    import serve_batch as sb
+    from lumina_b200 import cuda
+    model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], n_pages=8)
+    model.grow = lambda r, n: setattr(r, "pages", [10 ** 6] * 10)
+    r = sb.Request([1] * rows)
+    with pytest.raises(RuntimeError, match="fault word 64"):
+        model.serve([r], chunk=64)
+    assert r.out == [] and cuda.fault_status(0) == 0
