@@ -30,7 +30,7 @@ from lumina_b200.engine import rope_tables  # noqa: E402
 from lumina_b200.loader import LuminaFile, upload_record  # noqa: E402
 
 
-@dataclass
+@dataclass(eq=False)  # a request is itself, not its fields
 class Request:
     prompt: list
     max_tokens: int = 32

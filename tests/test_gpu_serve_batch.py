@@ -125,3 +125,18 @@ def test_a_step_with_a_fault_gives_no_tokens(tiny_file, rows):
     with pytest.raises(RuntimeError, match="fault word 64"):
         model.serve([r], chunk=64)
     assert r.out == [] and cuda.fault_status(0) == 0
+
+
+def test_requests_of_equal_fields(tiny_file):
+    """The same prompt twice, under different masks: each ends by itself."""
+    import serve_batch as sb
+    model = sb.BatchModel(tiny_file, CFG["num_attention_heads"], CFG["num_key_value_heads"], CFG["rope_theta"], n_pages=16)
+    masks = np.zeros((2, CFG["vocab_size"]), bool)
+    masks[0, 5] = masks[1, 9] = True
+    out = model.serve([sb.Request([1, 2, 3], max_tokens=2, allowed=m) for m in masks])
+    assert out == [[5, 5], [9, 9]]
+    assert not (sb.Request([1], allowed=masks[0]) == sb.Request([1], allowed=masks[1]))
+    one, two = sb.Request([1]), sb.Request([1])
+    live = [one, two]
+    live.remove(two)
+    assert live[0] is one
