@@ -62,7 +62,9 @@ class BatchModel:
                 return torch.tensor(recs[name].data, device=self.device)
 
             self.embed = raw("model.embed_tokens.weight").half()
-            self.head = raw("lm_head.weight").half() if "lm_head.weight" in recs else self.embed
+            # fp16 values as in the single-sequence model, whose head kernel has
+            # no entry of its own: an fp32 product of the library's
+            self.head = (raw("lm_head.weight").half() if "lm_head.weight" in recs else self.embed).float().T
             self.layers = []
             while "model.layers.%d.input_layernorm.weight" % len(self.layers) in recs:
                 p = "model.layers.%d." % len(self.layers)
@@ -116,7 +118,7 @@ class BatchModel:
             self._project(w["down"], torch.nn.functional.silu(ff[0]) * ff[1], y)
             x += y
         # no norm before the head, as in the single-sequence model
-        return x[torch.tensor(last, dtype=torch.long, device=self.device)] @ self.head.float().T
+        return x[torch.tensor(last, dtype=torch.long, device=self.device)] @ self.head
 
     def grow(self, r, tokens):
         while len(r.pages) * self.page_size < tokens:
