@@ -2,9 +2,11 @@
 // the choice between the two kernels.
 //
 // A sequence of few packed rows (new rows x query heads per KV head) is bound
-// by its cache's bytes and goes to the decode kernel (kvq_decode.cu), in up to
-// three (fp32 rows: four) tasks of 16 rows per KV head; one of more rows goes
-// to the chunk kernel (kvq_chunk.cu), bound by its tensor and softmax work.
+// by reading its cache and goes to the decode kernel (kvq_decode.cu), in tasks
+// of up to 16 packed rows per KV head; one of more than 48 (fp32 rows: 64)
+// goes to the chunk kernel (kvq_chunk.cu), bound by its softmax work. A task
+// holds whole rows, so where the heads do not divide 16 there are more tasks
+// than 48 / 16, and the decode kernel is still the faster one (below).
 // Each kernel takes its own sequences out of the batch, so a batch may mix
 // them. Decode / chunk kernel, int8, head dim 128, 8 KV heads, lengths up to
 // 4096, fp16 rows unless said:
@@ -12,6 +14,9 @@
 //   8 sequences,  64 packed rows     57 /  58 us, fp32 rows 64 / 75 us
 //   32 sequences, 32 packed rows     95 / 128 us
 //   32 sequences, 64 packed rows    171 / 133 us
+//   8 sequences x 5 rows of 9 heads 40 / 50 us (4 KV heads; five tasks of a row)
+//   8 sequences x 4 rows of 12 heads 31 / 47 us (2 KV heads; four tasks)
+//   8 sequences x 16 rows of 3 heads 50 / 58 us (four tasks of up to 5 rows)
 // Sequences for the decode kernel take at least a cell per warp and CTA
 // (1 x 640 tokens, 32 KV heads: 12.3 us; 14.4 with two cells, 16.4 with three).
 // Beside a sequence for the chunk kernel the others mostly bring one row, so

@@ -10,7 +10,7 @@ namespace lumina {
 constexpr int KVQ_MAX_CTAS = 512;    // CTAs that may leave partial states (two each)
 constexpr int KVQ_FAN = 64;          // partial states that one CTA joins at a time
 constexpr int KVQ_DECODE_ROWS = 16;  // packed rows of a decode task at most
-constexpr int KVQ_DECODE_BLOCKS = 4;  // tasks of one sequence and KV head at most
+constexpr int KVQ_DECODE_BLOCKS = 4;  // times so many: a sequence's packed rows for the decode kernel at most (fp32 rows)
 
 struct AttendArgs {
   KvqView v;

@@ -221,7 +221,7 @@ struct CkLine {
   const AttendArgs& a;
   const int *line, *blocks;
   int NBt, Tn;
-  unsigned share, u0, u1;
+  unsigned u0, u1;
   bool whole;
 };
 
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
     NBt = kvq_sum(NBt, total);
   }
   __syncthreads();
-  CkLine ln{a, line, blocks, 0, 0, 0u, 0u, 0u, false};
+  CkLine ln{a, line, blocks, 0, 0, 0u, 0u, false};
   ln.NBt = NBt;
   const bool whole = ln.whole = NBt > KVQ_MAX_BLOCKS;  // whole tasks: the line does not hold them
   int Tn = NBt;                             // units of one KV head: tiles, or tasks
@@ -379,7 +379,6 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
   // units [u0, u1), or tasks u0, u0 + gridDim.x, ...
   const unsigned u0 = whole ? blockIdx.x : min(U, blockIdx.x * share), u1 = whole ? U : min(U, u0 + share);
   ln.Tn = Tn;
-  ln.share = share;
   ln.u0 = u0;
   ln.u1 = u1;
   auto segment = [&](unsigned u, CkSeg& x) { return ck_segment<BM>(ln, u, x); };  // returns the next segment's unit

@@ -44,7 +44,7 @@ namespace lumina {
 
 namespace {
 
-template <int HD, int BITS, int NR, bool F32>
+template <int HD, int BITS, int NR>
 struct DecCfg {
   using F = KvqFrag<HD, BITS>;
   static constexpr int NK = NR == 2 && HD == 128 ? 1 : 2;  // 16-key tiles of one cell
@@ -56,9 +56,8 @@ struct DecCfg {
   static constexpr int R = 8 * NR;                          // packed rows
   static constexpr int LD = HD + 4;
   static constexpr int SLAB = R * LD * 4;                   // one warp's O
-  // joining parts: 4-dim items of a row, Q threads per item, weights and sums
-  static constexpr int ITEMS = R * (HD / 4), Q = THREADS / ITEMS > 0 ? THREADS / ITEMS : 1;
-  static constexpr int JOIN = (R * KVQ_FAN + (Q - 1) * ITEMS * 4) * 4;
+  static constexpr int ITEMS = R * (HD / 4);                // 4-dim items that join parts
+  static constexpr int JOIN = R * KVQ_FAN * 4;              // the parts' weights
   static constexpr int SMEM = W * SLAB > JOIN ? W * SLAB : JOIN;  // + n_seq ints
 };
 
@@ -71,10 +70,9 @@ struct Seg {
 };
 
 template <int HD, int BITS, int NR, typename T, bool PLAIN>
-__global__ void __launch_bounds__((DecCfg<HD, BITS, NR, sizeof(T) == 4>::THREADS), (DecCfg<HD, BITS, NR, sizeof(T) == 4>::PER_SM))
-kvq_decode_kernel(AttendArgs a) {
+__global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, BITS, NR>::PER_SM)) kvq_decode_kernel(AttendArgs a) {
   constexpr bool F32 = sizeof(T) == 4;
-  using C = DecCfg<HD, BITS, NR, F32>;
+  using C = DecCfg<HD, BITS, NR>;
   using F = typename C::F;
   constexpr int KK = F::KK, NT = F::NT, W = C::W, R = C::R, NK = C::NK, CELL = C::CELL;
   // fp16 rows spend next to no instructions on making numbers of the codes: K
@@ -661,27 +659,17 @@ kvq_decode_kernel(AttendArgs a) {
           }
         }
         __syncthreads();
-        // thread: 4 dims of a row, every Q-th part; the Q sums join in order
-        constexpr int ITEMS = C::ITEMS, Q = C::Q;
-        float* join = slab + R * KVQ_FAN;  // past the weights
-        for (int i0 = 0; i0 < ITEMS * Q; i0 += C::THREADS) {
-          const int i = (i0 + tid) % ITEMS, q = (i0 + tid) / ITEMS, r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        // thread: 4 dims of a row, the parts in order
+        static_assert(C::ITEMS % C::THREADS == 0, "whole passes of the CTA");
+        for (int i = tid; i < C::ITEMS; i += C::THREADS) {
+          const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
           if (r < rows) {
 #pragma unroll 16
-            for (int k = q; k < cnt; k += Q) {
+            for (int k = 0; k < cnt; ++k) {
               const float4 z = __ldcg(reinterpret_cast<const float4*>(part_at(k) + (size_t)r * HD + d));
               const float f = wt[r * KVQ_FAN + k];
               y.x = fmaf(z.x, f, y.x); y.y = fmaf(z.y, f, y.y); y.z = fmaf(z.z, f, y.z); y.w = fmaf(z.w, f, y.w);
-            }
-          }
-          if constexpr (Q > 1) {
-            if (q) *reinterpret_cast<float4*>(join + ((q - 1) * ITEMS + i) * 4) = y;
-            __syncthreads();
-            if (q) continue;
-            for (int k = 1; k < Q; ++k) {
-              const float4 z = *reinterpret_cast<const float4*>(join + ((k - 1) * ITEMS + i) * 4);
-              y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
             }
           }
           if (r >= rows) continue;
@@ -701,7 +689,7 @@ kvq_decode_kernel(AttendArgs a) {
 
 template <int HD, int BITS, int NR, typename T>
 int decode_nr(const AttendArgs& a, cudaStream_t s) {
-  using C = DecCfg<HD, BITS, NR, sizeof(T) == 4>;
+  using C = DecCfg<HD, BITS, NR>;
   auto kern = a.cap > 0.f || a.slopes ? kvq_decode_kernel<HD, BITS, NR, T, false> : kvq_decode_kernel<HD, BITS, NR, T, true>;
   const size_t smem = C::SMEM + (size_t)a.v.n_seq * 4;
   const int rc = set_smem_limit((const void*)kern, C::SMEM + KVQ_MAX_SEQ * 4, "kvq_decode");

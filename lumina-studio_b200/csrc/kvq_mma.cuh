@@ -1,19 +1,20 @@
-// Warp-level pieces of the attention over quantized KV pages on mma.sync
-// m16n8k16: 16 query rows x 16 keys per step, codes straight from memory to
-// fragments.
+// Pieces of the attention over quantized KV pages: codes to fragments of
+// mma.sync m16n8k16 (the decode kernel) and to fp16 numbers, the exponential
+// and tanh, and the sizes of V scales (both kernels).
 //
-// A warp step scores 16 packed query rows (row r = local row r / G, head r %
-// G of one KV head's G query heads) against 16 keys. Codes are small
-// integers, exact in fp16, so K and V enter the tensor pipe as they are
-// stored and the scales stay outside the products: a key's K scale
-// multiplies its score column, its V scale multiplies its probability.
+// The decode kernel's products are transposed, S^T = K Q^T and O^T = V^T P^T:
+// 16 keys (dims) fill a fragment's rows, up to 8 packed query rows (row r =
+// local row r / G, head r % G of one KV head's G query heads) its columns.
+// Codes are small integers, exact in fp16, so K and V enter the tensor pipe as
+// they are stored and the scales stay outside the products: a key's K scale
+// multiplies its scores, its V scale its probabilities.
 //
-// Fragment layouts (lane = 4 g + t): in the K fragment of key g, a thread's
-// four k-indices of a step are any four dims as long as q uses the same, so
-// thread t owns runs of the key's codes that load as 16-byte words
-// (load_q takes q's dims in that order). In the V fragment, n-tile i takes dim g * HD / 8 + i at column
-// g, so a thread loads one contiguous run per key and ends with the 2 HD / 8
-// contiguous output dims from 2 t HD / 8 on.
+// Fragment layouts (lane = 4 g + t): a thread's four k-indices of a step may
+// be any four dims of key g as long as q uses the same, so thread t owns runs
+// of the key's codes that load as 16-byte words (load_q takes q's dims in that
+// order). In V^T, row g of 8-dim tile i is dim g * HD / 8 + i, so a thread
+// loads one contiguous run per key and ends with HD / 8 contiguous dims of its
+// two output columns.
 #pragma once
 #include "kvq.cuh"
 
