@@ -374,3 +374,26 @@ def test_tensors_of_too_few_dims_are_refused(sv):
                  lambda: sv.adjust_logits(logits, mask=torch.zeros(4, dtype=torch.int32, device="cuda"))):
         with pytest.raises(LuminaError):
             call()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_joins_of_many_parts_fp16(sv, bits):
+    """More parts than one join takes, with fp16 rows."""
+    got, want = run_attend(sv, bits, 128, "float16", 8, 1, 64, [1], [40003], seed=91)
+    check_attend(got, want, "float16")
+
+
+@pytest.mark.parametrize("io", ["float16", "float32"])
+@pytest.mark.parametrize("cap,alibi,window,prefix", [
+    (0.0, True, 0, None),
+    (30.0, True, 70, [3, 200, 0, 5, 1000]),
+    (0.0, False, 64, [64, 65, 1, 0, 400]),
+    (0.0, False, 0, [900, 0, 63, 7, 900]),
+])
+@pytest.mark.parametrize("rows,lens", [
+    ([1, 1, 1, 1, 1], [1, 500, 64, 129, 900]),
+    ([1, 33, 2, 1, 200], [700, 300, 64, 129, 900]),
+])
+def test_masks_int4(sv, io, cap, alibi, window, prefix, rows, lens):
+    got, want = run_attend(sv, 4, 64, io, 6, 2, 16, rows, lens, cap, alibi, window, prefix, seed=92)
+    check_attend(got, want, io)
