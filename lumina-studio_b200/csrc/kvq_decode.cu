@@ -80,7 +80,10 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
   // points come off again, K's as a start value of the accumulator, V's by one
   // more product. q is exact (to 2^-35 of its largest value) and the sums are
   // fp32 over terms of up to twice the codes' size, so a score is right to
-  // about 2^-22 of sum |q k|. fp32 rows use signed codes and split q and p.
+  // about 2^-22 of sum |q k|. fp32 rows use signed codes and q as two fp16
+  // parts. p is two fp16 parts for either: one alone would add 2.0e-4 of the
+  // output to the 2.1e-4 of its rounding to fp16 (64 sequences of up to 8192:
+  // 90 us, 89 with one part; 8 x 5 drafts 40, 39).
   constexpr bool FAST = !F32;
   // a chunk kernel of the same call may take the SMs that this one leaves
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
     float m[NR][2], l[NR][2], ms[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = ms[r][0] = ms[r][1] = 0.f;
-    const float sign = FAST && (g & 1) ? -1.f : 1.f;  // odd keys' p (v_raw)
+    const float sign = FAST && (g & 1) ? -1.f : 1.f;  // odd keys' p (v_frag)
 
     // cells that start in [in_lo, in_hi] are seen by every row, as are those
     // that end within the prefix
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
           }
         }
       }
-      uint32_t pt[NK][NR][2], ptl[F32 ? NK : 1][F32 ? NR : 1][2];
+      uint32_t pt[NK][NR][2], ptl[NK][NR][2];  // p's fp16 parts
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         const float vs[2] = {sv[n][0] * sign, sv[n][1] * sign};
@@ -488,13 +491,9 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if constexpr (F32) {
-              uint32_t lo;
-              pt[n][r][h] = transpose8(split_h2(p[n][r][2 * h], p[n][r][2 * h + 1], lo));
-              ptl[n][r][h] = transpose8(lo);
-            } else {
-              pt[n][r][h] = transpose8(half2_bits(__floats2half2_rn(p[n][r][2 * h], p[n][r][2 * h + 1])));
-            }
+            uint32_t lo;
+            pt[n][r][h] = transpose8(split_h2(p[n][r][2 * h], p[n][r][2 * h + 1], lo));
+            ptl[n][r][h] = transpose8(lo);
           }
         }
       }
@@ -506,21 +505,13 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
         for (int w = 0; w < F::VW; ++w)
           static_for<DPW / 2>([&](auto ic) {
             constexpr int i = 2 * decltype(ic)::value;
-            if constexpr (FAST) {
-              const uint32_t f[4] = {
-                  F::template v_raw<i>(vw[n][0][w], vw[n][1][w]), F::template v_raw<i + 1>(vw[n][0][w], vw[n][1][w]),
-                  F::template v_raw<i>(vw[n][2][w], vw[n][3][w]), F::template v_raw<i + 1>(vw[n][2][w], vw[n][3][w])};
+            const uint32_t f[4] = {
+                F::template v_frag<i, FAST>(vw[n][0][w], vw[n][1][w]), F::template v_frag<i + 1, FAST>(vw[n][0][w], vw[n][1][w]),
+                F::template v_frag<i, FAST>(vw[n][2][w], vw[n][3][w]), F::template v_frag<i + 1, FAST>(vw[n][2][w], vw[n][3][w])};
 #pragma unroll
-              for (int r = 0; r < NR; ++r) mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
-            } else {
-              const uint32_t f[4] = {
-                  F::template v_pair<i>(vw[n][0][w], vw[n][1][w]), F::template v_pair<i + 1>(vw[n][0][w], vw[n][1][w]),
-                  F::template v_pair<i>(vw[n][2][w], vw[n][3][w]), F::template v_pair<i + 1>(vw[n][2][w], vw[n][3][w])};
-#pragma unroll
-              for (int r = 0; r < NR; ++r) {
-                mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
-                mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
-              }
+            for (int r = 0; r < NR; ++r) {
+              mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
+              mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
             }
           });
       if constexpr (FAST) {
@@ -528,7 +519,10 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) mma_16816(oz[r], f, pt[n][r][0], pt[n][r][1]);
+          for (int r = 0; r < NR; ++r) {
+            mma_16816(oz[r], f, ptl[n][r][0], ptl[n][r][1]);
+            mma_16816(oz[r], f, pt[n][r][0], pt[n][r][1]);
+          }
       }
       load_v();
     }

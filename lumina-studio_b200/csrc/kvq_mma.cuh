@@ -188,28 +188,22 @@ struct KvqFrag {
     }
   }
   // fp16 pairs (key a, key b) of dims DPW * j + i of the thread's run, where
-  // word j of each key holds DPW = 32 / BITS dims: c (int8), 2 c - 15 (int4)
-  template <int i>
-  __device__ static __forceinline__ uint32_t v_pair(uint32_t a, uint32_t b) {
-    if constexpr (BITS == 8) {
+  // word j of each key holds DPW = 32 / BITS dims: c (int8) or 2 c - 15 (int4).
+  // RAW (as in k_frag): the odd key's codes are complemented, to be met by a
+  // negated p; for odd i int4 codes come times 16.
+  static constexpr float RAW_ZERO[2] = {BITS == 8 ? 128.f : 7.5f, BITS == 8 ? 127.f : 7.5f};
+  template <int i, bool RAW>
+  __device__ static __forceinline__ uint32_t v_frag(uint32_t a, uint32_t b) {
+    if constexpr (BITS == 8 && RAW) {
+      const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7632 : 0x5410);  // a_i' a_i'+1 | b_i' b_i'+1
+      return (((i & 1) ? x >> 8 : x) ^ 0x007F0080u) & 0x00FF00FFu;
+    } else if constexpr (BITS == 8) {
       const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7362 : 0x5140);  // a_i' b_i' a_i'+1 b_i'+1
       return s8_pair<(i & 1) ? 0x4342 : 0x4140>(x ^ 0x80808080u);
     } else {
       const uint32_t x = __byte_perm(a, b, (i & 4) ? 0x7632 : 0x5410);
-      return u4_pair((i & 3) == 0 ? x << 4 : x >> (4 * ((i & 3) - 1)));
-    }
-  }
-  // The same pairs raw (as in k_frag), the odd key's codes complemented and
-  // to be met by a negated p; for odd i int4 codes come times 16.
-  static constexpr float RAW_ZERO[2] = {BITS == 8 ? 128.f : 7.5f, BITS == 8 ? 127.f : 7.5f};
-  template <int i>
-  __device__ static __forceinline__ uint32_t v_raw(uint32_t a, uint32_t b) {
-    if constexpr (BITS == 8) {
-      const uint32_t x = __byte_perm(a, b, (i & 2) ? 0x7632 : 0x5410);  // a_i' a_i'+1 | b_i' b_i'+1
-      return (((i & 1) ? x >> 8 : x) ^ 0x007F0080u) & 0x00FF00FFu;
-    } else {
-      const uint32_t x = __byte_perm(a, b, (i & 4) ? 0x7632 : 0x5410);
-      return (((i & 2) ? x >> 8 : x) ^ 0xFFFF0000u) & ((i & 1) ? 0x00F000F0u : 0x000F000Fu);
+      if constexpr (RAW) return (((i & 2) ? x >> 8 : x) ^ 0xFFFF0000u) & ((i & 1) ? 0x00F000F0u : 0x000F000Fu);
+      else return u4_pair((i & 3) == 0 ? x << 4 : x >> (4 * ((i & 3) - 1)));
     }
   }
 };

@@ -397,3 +397,13 @@ def test_joins_of_many_parts_fp16(sv, bits):
 def test_masks_int4(sv, io, cap, alibi, window, prefix, rows, lens):
     got, want = run_attend(sv, 4, 64, io, 6, 2, 16, rows, lens, cap, alibi, window, prefix, seed=92)
     check_attend(got, want, io)
+
+
+@pytest.mark.parametrize("bits,hd,page", [(8, 128, 16), (8, 64, 32), (4, 128, 64), (4, 64, 16)])
+@pytest.mark.parametrize("rows,lens", [([1] * 12, [1, 2, 3, 5, 17, 40, 100, 300, 700, 1000, 2000, 3000]), ([5, 3, 2], [6, 900, 40])])
+def test_decode_rows_are_rounded_once(sv, bits, hd, page, rows, lens):
+    """fp16 rows of the decode kernel are the definition rounded to fp16, but
+    for values within about 1e-6 of a tie: one in 250 off by 2^-10 at most,
+    6e-5 of the norm; 1e-4 is asked."""
+    got, want = run_attend(sv, bits, hd, "float16", 8, 2, page, rows, lens, seed=93)
+    assert rel(got, want.astype(np.float16)) < 1e-4
