@@ -10,7 +10,10 @@
 // K and V codes are small integers, exact in fp16; the scales stay outside:
 // a key's K scale multiplies its score column, its V scale its probability.
 // fp32 rows send Q and P as two fp16 parts (hi + lo, about 22 bits) through
-// the same tiles.
+// the same tiles. fp16 rows keep one part of P: its rounding adds 2.0e-4 of the
+// output to the 2.1e-4 of the output's own, and the second part costs a third
+// of the speed (2048 rows behind 14K tokens: 1118 us, 823 with one), most of it
+// in the softmax warps, whose 128 registers do not hold both.
 //
 // One CTA per SM, 13 warps:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: a thread is a row, so
@@ -33,11 +36,15 @@
 // CTAs take whole tasks instead.
 //
 // Bound by the softmax warps, whose pass over a tile takes longer than the
-// products it overlaps. 2048 rows behind 14K cached tokens, 32 / 8 heads of
-// 128, int8, fp16 rows: 822 us, 625 TFLOP/s (0.38 of the bf16 peak). The
-// loops' code size matters: the same with its helpers inline, twice the text,
-// was 10 % slower. 285 rows of 28 / 4 heads of 64 over 4096 int4 keys, fp32
-// rows with cap, distance bias, window and prefix: 63 us.
+// products it overlaps: by latency, with the tensor pipe at 29 % and 1.6
+// instructions a cycle of 4. Two of them per scheduler walk two dependent
+// passes over S in tensor memory (maximum, then exponentials), and 13 warps
+// leave a thread 128 registers, which neither pass's next columns fit beside.
+// 2048 rows behind 14K cached tokens, 32 / 8 heads of 128, int8, fp16 rows: 823
+// us, 625 TFLOP/s (0.38 of the bf16 peak); 1024 fp32 rows behind 7K: 416 us.
+// The loops' code size matters: the same with its helpers inline, twice the
+// text, was 10 % slower. 285 rows of 28 / 4 heads of 64 over 4096 int4 keys,
+// fp32 rows with cap, distance bias, window and prefix: 63 us.
 //
 // Waits are bounded: one that gives up sets bit 5 of the device fault word,
 // every role leaves its loop, its rows stay unwritten (whoever joins their

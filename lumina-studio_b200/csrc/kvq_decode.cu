@@ -1,5 +1,5 @@
 // Attention of sequences with few new rows (decode steps, short drafts) over
-// quantized KV pages: bound by the bytes of the cache.
+// quantized KV pages.
 //
 // A task is one (KV head, sequence, block of its new rows): up to 8 NR packed
 // query rows (row r = local row r / G, head r % G); the blocks of one
@@ -23,17 +23,18 @@
 // nothing from the others); it moves only when a key passes it by 2^8, so the
 // steady state has no shuffles.
 //
-// Measured: 64 sequences of up to 8192 tokens, 32 / 8 heads of 128, int8, fp16
-// rows: 87 us, 0.71 of the copy rate; 2 sequences of up to 131072, 32 / 4
-// heads, int4: 60 us, bound by the chain of a cell's math (two warps per
-// scheduler issue 0.3 instructions a cycle; about 600 per cell); one of
-// 640 tokens, 32 / 32 heads, fp32 rows: 12.3 us. CTAs of four warps, two per SM:
+// Bound by the chain of a cell's math, from scores through exponentials to the
+// second product: two warps per scheduler (a warp's registers hold a cell's
+// codes and the output) issue 0.3 instructions a cycle, with DRAM at 27 to 45 %
+// and the tensor pipe at 17 to 19 %. 64 sequences of up to 8192 tokens, 32 / 8
+// heads of 128, int8, fp16 rows: 90 us, 0.69 of the copy rate (fp32 rows 97); 2
+// sequences of up to 131072, 32 / 4 heads, int4: 62 us, 0.35 of it; one of 640
+// tokens, 32 / 32 heads, fp32 rows: 12.4 us. CTAs of four warps, two per SM:
 // one merges and joins while the other streams. A third CTA per SM spills at
 // head dim 128 (the 64 sequences: 118 us).
 //
 // tcgen05 would need the codes rewritten as fp16 in shared memory and 128
-// rows where these sequences have at most 8 NR; the cache's bytes bound this
-// kernel well before the tensor pipe does.
+// rows where these sequences have at most 8 NR.
 #include <cfloat>
 #include <type_traits>
 
