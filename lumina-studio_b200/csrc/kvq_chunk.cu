@@ -73,6 +73,13 @@ template <bool F32>
 struct CkLift {
   static constexpr float LIFT = F32 ? 5.f : -2.f, MARGIN = 15.f - LIFT;
 };
+// The tensor pipe cuts its sums off instead of rounding them, which over
+// thousands of keys shrinks an fp32 output by several 1e-6 (8 sequences x 256
+// rows of 8192 keys: an error of 5.6e-6). A softmax group of fp32 rows takes O
+// out of tensor memory after every CK_SUM of its tiles and adds it to a sum in
+// the workspace, rounded.
+// (1024 rows behind 7K tokens: 441 us, 414 without.)
+constexpr int CK_SUM = 8;
 constexpr int CK_TILE = 128 * 128;          // bytes of a [128 rows][64 fp16] block
 constexpr uint32_t CK_S = 0, CK_O = 256;    // tensor memory columns: S tiles, O tiles, 128 apart
 
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           ck_fence_after();
           const uint64_t vd = ck_desc(sb + C::OFF_V + st * C::BYTES, CK_TILE);
           const uint32_t d = tm + CK_O + t * 128, p = tm + CK_S + t * 128;
-          const int fresh = j < 2;  // the group's first tile: O starts here
+          const int fresh = F32 ? (j >> 1) % CK_SUM == 0 : j < 2;  // O starts here
           if (lead) {
 #pragma unroll
             for (int part = 0; part < (F32 ? 2 : 1); ++part)
@@ -686,6 +693,21 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       const int r_lo = a.window ? pos - a.window + 1 : 0, r_hi = min(pos, x.len - 1);  // sees r_lo .. r_hi and 0 .. pre - 1
       // m: the largest score plus V scale's size when the reference last moved
       float m = -INFINITY, l = 0.f, ref = 0.f;
+      // fp32 rows: the sum of earlier O tiles, relative to 2^sum_ref (-inf:
+      // nothing seen yet); behind the parts (a slot holds 128 of its 256 rows)
+      float sum_ref = -INFINITY;
+      bool summed = false;
+      auto against = [](float r, float top) { return r == -INFINITY ? 0.f : ex2(r - top); };
+      float4* sum_at = reinterpret_cast<float4*>(a.ws + (size_t)2 * KVQ_CHUNK_CTAS * BM * (HD + 2)) +
+                       (size_t)(2 * blockIdx.x + t) * 128 * (HD / 4) + row;
+      auto add_sum = [&](int c, float (&o)[32], float fo, float fs) {  // columns 32 c .. of O and of the sum
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 z = __ldcg(sum_at + (8 * c + i) * 128);
+          o[4 * i] = fmaf(z.x, fs, o[4 * i] * fo); o[4 * i + 1] = fmaf(z.y, fs, o[4 * i + 1] * fo);
+          o[4 * i + 2] = fmaf(z.z, fs, o[4 * i + 2] * fo); o[4 * i + 3] = fmaf(z.w, fs, o[4 * i + 3] * fo);
+        }
+      };
       const int J = x.alt ? nt : 2 * nt;
 #pragma unroll 1
       for (int j = t; j < J && !dead; j += 2) {
@@ -775,13 +797,27 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           }
           if constexpr (GC == 32) ck_wait_st();
         }
+        if (F32 && j >= 2 && (j >> 1) % CK_SUM == 0) {  // (the products of O's tiles are done, as below)
+          const float own = m == -INFINITY ? m : ref, top = fmaxf(sum_ref, own), fo = against(own, top), fs = against(sum_ref, top);
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            float o[32];
+            ck_get32(o_tm + 32 * c, o);
+            if (summed) add_sum(c, o, fo, fs);  // (else fo is 1, or O is 0)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) __stcg(sum_at + (8 * c + i) * 128, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+          }
+          sum_ref = top;
+          summed = true;
+        }
         if (__any_sync(0xffffffffu, mx > hold)) {
           const float rn = (mx == -INFINITY ? 0.f : mx) - CkLift<F32>::LIFT;
           const float fac = m == -INFINITY ? 0.f : ex2(ref - rn);
           m = mx;
           ref = rn;
           l *= fac;
-          if (j >= 2) {  // O holds this group's earlier tiles (their products are done: S of this tile came after them)
+          // O holds this group's earlier tiles (their products are done: S of this tile came after them)
+          if (F32 ? (j >> 1) % CK_SUM != 0 : j >= 2) {
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
               float o[32];
@@ -883,6 +919,17 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       }
       if (mine) ++no;
       dead |= !have;
+      // O of the whole segment, relative to 2^ref, columns 32 c ..
+      const float own = m == -INFINITY ? m : ref, whole_ref = fmaxf(sum_ref, own);
+      const float end_o = against(own, whole_ref), end_s = against(sum_ref, whole_ref);
+      auto get_o = [&](int c, float (&o)[32]) {
+        ck_get32(o_tm + 32 * c, o);
+        if (F32 && summed) add_sum(c, o, end_o, end_s);
+      };
+      if (F32 && summed) {
+        l *= end_o;
+        ref = whole_ref;
+      }
       float* merge = reinterpret_cast<float*>(sm);  // the Q tiles are free: [128 rows][HD] floats, 16-byte chunks swizzled
       auto at = [&](int r, int c4) { return reinterpret_cast<float4*>(merge + r * HD) + (c4 ^ (r & (HD / 4 - 1))); };
       float f1 = 1.f;  // this group's weight (alternating: against the other's)
@@ -894,7 +941,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
               float o[32];
-              ck_get32(o_tm + 32 * c, o);
+              get_o(c, o);
 #pragma unroll
               for (int i = 0; i < 8; ++i) *at(row, 8 * c + i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             }
@@ -942,7 +989,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           float o[32];
-          ck_get32(o_tm + 32 * c, o);
+          get_o(c, o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= f1;
           if (other) {

@@ -500,21 +500,51 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
       }
       load_s();
       constexpr int DPW = 32 / BITS;  // dims per code word
+      if constexpr (FAST) {
 #pragma unroll
-      for (int n = 0; n < NK; ++n)
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int w = 0; w < F::VW; ++w)
+            static_for<DPW / 2>([&](auto ic) {
+              constexpr int i = 2 * decltype(ic)::value;
+              const uint32_t f[4] = {
+                  F::template v_frag<i, true>(vw[n][0][w], vw[n][1][w]), F::template v_frag<i + 1, true>(vw[n][0][w], vw[n][1][w]),
+                  F::template v_frag<i, true>(vw[n][2][w], vw[n][3][w]), F::template v_frag<i + 1, true>(vw[n][2][w], vw[n][3][w])};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
+                mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
+              }
+            });
+      } else {
+        // The tensor pipe cuts its sums off instead of rounding them, which
+        // over thousands of keys shrinks an fp32 output by several 1e-6. A
+        // cell's sums start at 0 and join the others by rounded additions (64
+        // sequences of up to 8192: 106 us, 97 without).
 #pragma unroll
         for (int w = 0; w < F::VW; ++w)
           static_for<DPW / 2>([&](auto ic) {
             constexpr int i = 2 * decltype(ic)::value;
-            const uint32_t f[4] = {
-                F::template v_frag<i, FAST>(vw[n][0][w], vw[n][1][w]), F::template v_frag<i + 1, FAST>(vw[n][0][w], vw[n][1][w]),
-                F::template v_frag<i, FAST>(vw[n][2][w], vw[n][3][w]), F::template v_frag<i + 1, FAST>(vw[n][2][w], vw[n][3][w])};
+            float d[NR][4];
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              mma_16816(o[r][(w * DPW + i) / 2], f, ptl[n][r][0], ptl[n][r][1]);
-              mma_16816(o[r][(w * DPW + i) / 2], f, pt[n][r][0], pt[n][r][1]);
+            for (int r = 0; r < NR; ++r) d[r][0] = d[r][1] = d[r][2] = d[r][3] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+              const uint32_t f[4] = {
+                  F::template v_frag<i, false>(vw[n][0][w], vw[n][1][w]), F::template v_frag<i + 1, false>(vw[n][0][w], vw[n][1][w]),
+                  F::template v_frag<i, false>(vw[n][2][w], vw[n][3][w]), F::template v_frag<i + 1, false>(vw[n][2][w], vw[n][3][w])};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                mma_16816(d[r], f, ptl[n][r][0], ptl[n][r][1]);
+                mma_16816(d[r], f, pt[n][r][0], pt[n][r][1]);
+              }
             }
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[r][(w * DPW + i) / 2][e] += d[r][e];
           });
+      }
       if constexpr (FAST) {
         const uint32_t zp = half2_bits(__floats2half2_rn(F::RAW_ZERO[0], F::RAW_ZERO[1])), f[4] = {zp, zp, zp, zp};
 #pragma unroll

@@ -407,3 +407,37 @@ def test_decode_rows_are_rounded_once(sv, bits, hd, page, rows, lens):
     6e-5 of the norm; 1e-4 is asked."""
     got, want = run_attend(sv, bits, hd, "float16", 8, 2, page, rows, lens, seed=93)
     assert rel(got, want.astype(np.float16)) < 1e-4
+
+
+@pytest.mark.parametrize("n_seq,rows,hd,bits,tol", [
+    (16, 32, 64, 8, 4e-6), (8, 32, 128, 4, 4e-6),                         # the chunk kernel
+    (64, 1, 64, 8, 1e-6), (32, 1, 128, 8, 1e-6), (12, 4, 128, 4, 1e-6),   # the decode kernel
+])
+def test_fp32_sums_over_many_keys(sv, n_seq, rows, hd, bits, tol):
+    """Equal weights over 8192 positive values: the mean, for fp32 rows, with
+    work enough that one CTA sums hundreds of cells or tiles. The tensor pipe
+    cuts sums off, by 2^-24 of the sum so far on average at most, which is half
+    the whole on average: 128 such sums between two rounded additions cost 3.8e-6
+    (chunk kernel), four cost 1e-7 (decode kernel); the rounded additions of up
+    to 1000 parts sqrt(1000) 2^-25 = 9e-7."""
+    import torch
+    rng = np.random.default_rng(95)
+    ln, page, n_kv, G = 8192, 64, 8, 4
+    table, n_pages, _ = layout(rng, [ln] * n_seq, page)
+    nb = hd * bits // 8
+    gen = torch.Generator(device="cuda").manual_seed(n_seq)
+    data = torch.empty(n_pages, n_kv, ref.block_bytes(bits, hd, page), dtype=torch.uint8, device="cuda")
+    codes = torch.randint(64, 128, data[:, :, :2 * page * nb].shape, dtype=torch.uint8, device="cuda", generator=gen)
+    data[:, :, :2 * page * nb] = codes if bits == 8 else codes | 0x88  # int4: codes 8 .. 15, values 1 .. 15
+    scales = 1 + torch.rand(n_pages, n_kv, 2 * page, device="cuda", generator=gen)
+    data[:, :, 2 * page * nb:] = scales.view(torch.uint8)
+    q = torch.zeros(n_seq * rows, n_kv * G, hd, device="cuda")
+    got = sv.KVPool(data, bits, hd, page).attend(batch_of(sv, [rows] * n_seq, [ln] * n_seq, table), q).double()
+    for s in range(n_seq):
+        at = torch.from_numpy(table[s].astype(np.int64)).cuda()
+        raw = data[at][:, :, page * nb:2 * page * nb].reshape(-1, n_kv, page, nb)
+        v = raw.view(torch.int8).double() if bits == 8 else 2 * torch.stack((raw & 15, raw >> 4), -1).flatten(-2).double() - 15
+        v = (v * scales[at][:, :, page:].double()[..., None]).transpose(1, 2).reshape(ln, n_kv, hd)
+        want = v.cumsum(0)[ln - rows:] / torch.arange(ln - rows + 1, ln + 1, device="cuda", dtype=torch.float64)[:, None, None]
+        d = got[s * rows:(s + 1) * rows].view(rows, n_kv, G, hd) / want[:, :, None] - 1
+        assert d.square().mean().sqrt() < tol
