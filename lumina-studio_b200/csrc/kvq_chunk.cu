@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           float z[2][32];
           ck_ld32(s_tm, z[0]);
           const float2 nref = make_float2(-ref, -ref);
-          float2 l2[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
+          float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // of this tile: small weights would be lost beside the whole
 #pragma unroll 1
           for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
@@ -868,8 +868,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             ck_st16(s_tm + 32 * c, ph);
             if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
           }
-          l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+          l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
         } else {
+          float lt = 0.f;
 #pragma unroll 1
           for (int c = 0; c < 128 / GC; ++c) {
             float z[GC];
@@ -884,7 +885,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float y = ex2(z[4 * i + e] - ref);
-                l += y;
+                lt += y;
                 p[e] = z[4 * i + e] == -INFINITY ? 0.f : y * vs[e];  // a masked key counts for nothing, whatever its scale holds
               }
               if constexpr (F32) {
@@ -902,6 +903,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
             ck_put<GC / 2>(to, ph);
             if constexpr (F32) ck_put<GC / 2>(to + 16, pl);
           }
+          l += lt;
         }
         ck_wait_st();
         ck_fence_before();

@@ -478,6 +478,9 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
         }
       }
       uint32_t pt[NK][NR][2], ptl[NK][NR][2];  // p's fp16 parts
+      float lc[NR][2];  // sums of this cell's p: small ones would be lost beside the whole
+#pragma unroll
+      for (int r = 0; r < NR; ++r) lc[r][0] = lc[r][1] = 0.f;
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         const float vs[2] = {sv[n][0] * sign, sv[n][1] * sign};
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = p[n][r][e], y = ex2(x - ms[r][e & 1]);
-            l[r][e & 1] += y;
+            lc[r][e & 1] += y;
             // a masked key counts for nothing, whatever its scale holds
             p[n][r][e] = !inner && x == -INFINITY ? 0.f : y * vs[e >> 1];
           }
@@ -498,6 +501,8 @@ __global__ void __launch_bounds__((DecCfg<HD, BITS, NR>::THREADS), (DecCfg<HD, B
           }
         }
       }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) l[r][0] += lc[r][0], l[r][1] += lc[r][1];
       load_s();
       constexpr int DPW = 32 / BITS;  // dims per code word
       if constexpr (FAST) {

@@ -441,3 +441,27 @@ def test_fp32_sums_over_many_keys(sv, n_seq, rows, hd, bits, tol):
         want = v.cumsum(0)[ln - rows:] / torch.arange(ln - rows + 1, ln + 1, device="cuda", dtype=torch.float64)[:, None, None]
         d = got[s * rows:(s + 1) * rows].view(rows, n_kv, G, hd) / want[:, :, None] - 1
         assert d.square().mean().sqrt() < tol
+
+
+@pytest.mark.parametrize("n_seq,rows,hd,tol", [(16, 32, 64, 1e-5), (8, 32, 128, 1e-5), (64, 1, 64, 4e-6), (64, 1, 128, 4e-6)])
+def test_many_small_weights_beside_a_large_one(sv, n_seq, rows, hd, tol):
+    """The first key weighs 2^25 times each of 8191 others, which together weigh
+    2.4e-4 of it; all values are the same, so the output is that value. Added
+    one by one to the large weight the small ones would be lost; in sums of a
+    tile (2^-18) or of four (2^-23) they round at 2^-25: 64 times 2^-25 = 2e-6.
+    (The chunk kernel's products add 128 sums that are cut off: 2^-24 each on
+    average, 8e-6.)"""
+    import torch
+    ln, page, n_kv, G = 8192, 64, 8, 4
+    rng = np.random.default_rng(96)
+    table, n_pages, _ = layout(rng, [ln] * n_seq, page)
+    data = torch.full((n_pages, n_kv, ref.block_bytes(8, hd, page)), 127, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(n_pages, n_kv, 2 * page, device="cuda")
+    scales[:, :, page:] = 0.3 / 127
+    first = torch.from_numpy(table[:, 0].astype(np.int64)).cuda()
+    scales[first, :, 0] = 25 * np.log(2) / (127 * hd ** 0.5)  # q = 1: a score of 25 ln 2
+    data[:, :, 2 * page * hd:] = scales.view(torch.uint8)
+    q = torch.ones(n_seq * rows, n_kv * G, hd, device="cuda")
+    got = sv.KVPool(data, 8, hd, page).attend(batch_of(sv, [rows] * n_seq, [ln] * n_seq, table), q).double()
+    value = 127 * float(np.float32(0.3 / 127))
+    assert (got / value - 1).abs().max() < tol
