@@ -11,9 +11,9 @@
 // a key's K scale multiplies its score column, its V scale its probability.
 // fp32 rows send Q and P as two fp16 parts (hi + lo, about 22 bits) through
 // the same tiles. fp16 rows keep one part of P: its rounding adds 2.0e-4 of the
-// output to the 2.1e-4 of the output's own, and the second part costs a third
-// of the speed (2048 rows behind 14K tokens: 1118 us, 823 with one), most of it
-// in the softmax warps, whose 128 registers do not hold both.
+// output to the 2.1e-4 of the output's own, and the second part costs an eighth
+// of the speed (2048 rows behind 14K tokens: 928 us, 817 with one), most of it in
+// the softmax warps.
 //
 // One CTA per SM, 13 warps:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: a thread is a row, so
@@ -40,8 +40,8 @@
 // instructions a cycle of 4. Two of them per scheduler walk two dependent
 // passes over S in tensor memory (maximum, then exponentials), and 13 warps
 // leave a thread 128 registers, which neither pass's next columns fit beside.
-// 2048 rows behind 14K cached tokens, 32 / 8 heads of 128, int8, fp16 rows: 823
-// us, 625 TFLOP/s (0.38 of the bf16 peak); 1024 fp32 rows behind 7K: 416 us.
+// 2048 rows behind 14K cached tokens, 32 / 8 heads of 128, int8, fp16 rows: 817
+// us, 630 TFLOP/s (0.38 of the bf16 peak); 1024 fp32 rows behind 7K: 424 us.
 // The loops' code size matters: the same with its helpers inline, twice the
 // text, was 10 % slower. 285 rows of 28 / 4 heads of 64 over 4096 int4 keys,
 // fp32 rows with cap, distance bias, window and prefix: 63 us.
@@ -74,12 +74,12 @@ struct CkLift {
   static constexpr float LIFT = F32 ? 5.f : -2.f, MARGIN = 15.f - LIFT;
 };
 // The tensor pipe cuts its sums off instead of rounding them, which over
-// thousands of keys shrinks an fp32 output by several 1e-6 (8 sequences x 256
-// rows of 8192 keys: an error of 5.6e-6). A softmax group of fp32 rows takes O
-// out of tensor memory after every CK_SUM of its tiles and adds it to a sum in
-// the workspace, rounded.
-// (1024 rows behind 7K tokens: 441 us, 414 without.)
-constexpr int CK_SUM = 8;
+// thousands of keys shrinks an fp32 output by several 1e-6. A softmax group of
+// fp32 rows takes O out of tensor memory after every CK_SUM of its tiles and
+// adds it to a sum in the workspace, rounded (1024 rows behind 7K tokens: an
+// error of 9.6e-7 and 424 us; 1.7e-6 after every 8 tiles, 3 % faster; 4.8e-6 at
+// the end alone).
+constexpr int CK_SUM = 4;
 constexpr int CK_TILE = 128 * 128;          // bytes of a [128 rows][64 fp16] block
 constexpr uint32_t CK_S = 0, CK_O = 256;    // tensor memory columns: S tiles, O tiles, 128 apart
 
@@ -137,11 +137,22 @@ __device__ __forceinline__ void ck_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void ck_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 // the loads issued so far are in their registers; v may be used after this
-__device__ __forceinline__ void ck_wait_ld(float (&v)[32]) {
+template <int N>
+__device__ __forceinline__ void ck_wait_ld(float (&v)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 __device__ __forceinline__ void ck_get32(uint32_t addr, float (&v)[32]) {
   ck_ld32(addr, v);
@@ -176,6 +187,11 @@ __device__ __forceinline__ void ck_st16(uint32_t addr, const uint32_t (&r)[16]) 
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void ck_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void ck_st32(uint32_t addr, const float (&v)[32]) {
   asm volatile(
@@ -829,44 +845,71 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
           }
         }
         if (fast) {
-          float z[2][32];
-          ck_ld32(s_tm, z[0]);
           const float2 nref = make_float2(-ref, -ref);
           float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // of this tile: small weights would be lost beside the whole
-#pragma unroll 1
-          for (int c2 = 0; c2 < 4; c2 += 2)
+          auto weigh = [&](int q, const float* w, float2& u0, float2& u1) {  // keys 4 q .. + 3
+            const float4 k4 = ksc[q], v4 = vsc[q];
+            u0 = make_float2(w[0], w[1]);
+            u1 = make_float2(w[2], w[3]);
+            if constexpr (F32) {
+              u0 = mul2(u0, make_float2(rmul, rmul));
+              u1 = mul2(u1, make_float2(rmul, rmul));
+            }
+            u0 = fma2(u0, make_float2(k4.x, k4.y), nref);
+            u1 = fma2(u1, make_float2(k4.z, k4.w), nref);
+            u0.x = ex2(u0.x); u0.y = ex2(u0.y); u1.x = ex2(u1.x); u1.y = ex2(u1.y);
+            l2[0] = add2(l2[0], u0);
+            l2[1] = add2(l2[1], u1);
+            u0 = mul2(u0, make_float2(v4.x, v4.y));
+            u1 = mul2(u1, make_float2(v4.z, v4.w));
+          };
+          if constexpr (F32) {
+            // 16 keys at a time: two parts of 32 spill (461 us where this takes 424)
+            float za[16], zb[16];
+            uint32_t ph[8], pa[8], pb[8];
+            auto parts = [&](int c, const float (&z)[16], uint32_t (&lo)[8]) {  // keys 16 c ..
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = c2 + h;
-            ck_wait_ld(z[h]);
-            if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
-            float(&w)[32] = z[h];
-            uint32_t ph[16], pl[F32 ? 16 : 1];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 k4 = ksc[8 * c + i], v4 = vsc[8 * c + i];
-              float2 u0 = make_float2(w[4 * i], w[4 * i + 1]), u1 = make_float2(w[4 * i + 2], w[4 * i + 3]);
-              if constexpr (F32) {
-                u0 = mul2(u0, make_float2(rmul, rmul));
-                u1 = mul2(u1, make_float2(rmul, rmul));
+              for (int i = 0; i < 4; ++i) {
+                float2 u0, u1;
+                weigh(4 * c + i, z + 4 * i, u0, u1);
+                ph[2 * i] = split_h2(u0.x, u0.y, lo[2 * i]);
+                ph[2 * i + 1] = split_h2(u1.x, u1.y, lo[2 * i + 1]);
               }
-              u0 = fma2(u0, make_float2(k4.x, k4.y), nref);
-              u1 = fma2(u1, make_float2(k4.z, k4.w), nref);
-              u0.x = ex2(u0.x); u0.y = ex2(u0.y); u1.x = ex2(u1.x); u1.y = ex2(u1.y);
-              l2[0] = add2(l2[0], u0);
-              l2[1] = add2(l2[1], u1);
-              u0 = mul2(u0, make_float2(v4.x, v4.y));
-              u1 = mul2(u1, make_float2(v4.z, v4.w));
-              if constexpr (F32) {
-                ph[2 * i] = split_h2(u0.x, u0.y, pl[2 * i]);
-                ph[2 * i + 1] = split_h2(u1.x, u1.y, pl[2 * i + 1]);
-              } else {
+            };
+            ck_ld16(s_tm, za);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              ck_wait_ld(za);
+              ck_ld16(s_tm + 32 * c + 16, zb);
+              parts(2 * c, za, pa);
+              ck_st8(s_tm + 32 * c, ph);
+              ck_wait_ld(zb);
+              if (c < 3) ck_ld16(s_tm + 32 * (c + 1), za);
+              ck_st8(s_tm + 32 * c + 16, pa);  // over scores that are in registers now
+              parts(2 * c + 1, zb, pb);
+              ck_st8(s_tm + 32 * c + 8, ph);
+              ck_st8(s_tm + 32 * c + 24, pb);
+            }
+          } else {
+            float z[2][32];
+            ck_ld32(s_tm, z[0]);
+#pragma unroll 1
+            for (int c2 = 0; c2 < 4; c2 += 2)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c2 + h;
+              ck_wait_ld(z[h]);
+              if (c < 3) ck_ld32(s_tm + 32 * (c + 1), z[h ^ 1]);
+              uint32_t ph[16];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float2 u0, u1;
+                weigh(8 * c + i, z[h] + 4 * i, u0, u1);
                 ph[2 * i] = half2_bits(__floats2half2_rn(u0.x, u0.y));
                 ph[2 * i + 1] = half2_bits(__floats2half2_rn(u1.x, u1.y));
               }
+              ck_st16(s_tm + 32 * c, ph);
             }
-            ck_st16(s_tm + 32 * c, ph);
-            if constexpr (F32) ck_st16(s_tm + 32 * c + 16, pl);
           }
           l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
         } else {
