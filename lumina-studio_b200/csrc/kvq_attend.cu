@@ -10,16 +10,16 @@
 // Each kernel takes its own sequences out of the batch, so a batch may mix
 // them. Decode / chunk kernel, int8, head dim 128, 8 KV heads, lengths up to
 // 4096, fp16 rows unless said:
-//   8 sequences,  20 packed rows     39 /  57 us, fp32 rows 42 / 66 us
+//   8 sequences,  20 packed rows     39 /  57 us, fp32 rows 43 / 65 us
 //   8 sequences,  48 packed rows     50 /  59 us
-//   8 sequences,  64 packed rows     59 /  60 us, fp32 rows 65 / 75 us
+//   8 sequences,  64 packed rows     59 /  59 us, fp32 rows 67 / 72 us
 //   32 sequences, 32 packed rows    104 / 131 us
 //   32 sequences, 48 packed rows    146 / 136 us
-//   32 sequences, 64 packed rows    191 / 137 us, fp32 rows 211 / 168 us
-//   8 sequences x 5 rows of 9 heads  40 /  54 us (4 KV heads; five tasks of a row)
-//   8 sequences x 4 rows of 12 heads 32 /  53 us (2 KV heads; four tasks)
+//   32 sequences, 64 packed rows    190 / 136 us, fp32 rows 221 / 165 us
+//   8 sequences x 5 rows of 9 heads  40 /  59 us (4 KV heads; five tasks of a row)
+//   8 sequences x 4 rows of 12 heads 33 /  60 us (2 KV heads; four tasks)
 // Sequences for the decode kernel take at least a cell per warp and CTA
-// (1 x 640 tokens, 32 KV heads: 12.3 us; 14.4 with two cells, 16.4 with three).
+// (1 x 640 tokens, 32 KV heads: 12.4 us; 14.4 with two cells, 16.4 with three).
 // Beside a sequence for the chunk kernel the others mostly bring one row, so
 // the decode kernel's blocks are 8 rows there.
 #include <cmath>

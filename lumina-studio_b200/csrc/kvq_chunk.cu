@@ -43,8 +43,8 @@
 // 2048 rows behind 14K cached tokens, 32 / 8 heads of 128, int8, fp16 rows: 817
 // us, 630 TFLOP/s (0.38 of the bf16 peak); 1024 fp32 rows behind 7K: 424 us.
 // The loops' code size matters: the same with its helpers inline, twice the
-// text, was 10 % slower. 285 rows of 28 / 4 heads of 64 over 4096 int4 keys,
-// fp32 rows with cap, distance bias, window and prefix: 63 us.
+// text, was 10 % slower. 301 rows of 28 / 4 heads of 64 over 4096 int4 keys,
+// fp32 rows with cap, distance bias, window and prefix: 68 us.
 //
 // Waits are bounded: one that gives up sets bit 5 of the device fault word,
 // every role leaves its loop, its rows stay unwritten (whoever joins their

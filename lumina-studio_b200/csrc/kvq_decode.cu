@@ -27,7 +27,7 @@
 // second product: two warps per scheduler (a warp's registers hold a cell's
 // codes and the output) issue 0.3 instructions a cycle, with DRAM at 27 to 45 %
 // and the tensor pipe at 17 to 19 %. 64 sequences of up to 8192 tokens, 32 / 8
-// heads of 128, int8, fp16 rows: 90 us, 0.69 of the copy rate (fp32 rows 97); 2
+// heads of 128, int8, fp16 rows: 90 us, 0.69 of the copy rate (fp32 rows 106); 2
 // sequences of up to 131072, 32 / 4 heads, int4: 62 us, 0.35 of it; one of 640
 // tokens, 32 / 32 heads, fp32 rows: 12.4 us. CTAs of four warps, two per SM:
 // one merges and joins while the other streams. A third CTA per SM spills at
