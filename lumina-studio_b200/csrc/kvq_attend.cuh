@@ -41,8 +41,8 @@ constexpr int KVQ_MAX_BLOCKS = 2048;  // row blocks whose key tiles the chunk ke
 constexpr int KVQ_CHUNK_CTAS = 160;   // CTAs of the chunk kernel at most
 constexpr int KVQ_CHUNK_ROWS = 256;   // packed rows of its partial states
 
-// workspace: tickets, then partial states; the two kernels of a mixed batch
-// overlap, so each has its own of both
+// workspace: tickets, then partial states (and the chunk kernel's sums of fp32
+// rows); the two kernels of a mixed batch overlap, so each has its own of both
 constexpr size_t KVQ_WS_DECODE_TICKETS = 4 * KVQ_MAX_CTAS, KVQ_WS_CHUNK_TICKETS = 2 * KVQ_CHUNK_CTAS;
 constexpr size_t KVQ_WS_TICKETS = (KVQ_WS_DECODE_TICKETS + KVQ_WS_CHUNK_TICKETS) * sizeof(int);
 constexpr size_t KVQ_WS_DECODE = (size_t)KVQ_MAX_CTAS * 2 * KVQ_DECODE_ROWS * (128 + 2);  // floats

@@ -711,6 +711,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) kvq_chunk_kernel(const __grid_c
       float m = -INFINITY, l = 0.f, ref = 0.f;
       // fp32 rows: the sum of earlier O tiles, relative to 2^sum_ref (-inf:
       // nothing seen yet); behind the parts (a slot holds 128 of its 256 rows)
+      static_assert(!F32 || (size_t)2 * KVQ_CHUNK_CTAS * BM * (2 * HD + 2) <= KVQ_WS_CHUNK, "parts and sums");
       float sum_ref = -INFINITY;
       bool summed = false;
       auto against = [](float r, float top) { return r == -INFINITY ? 0.f : ex2(r - top); };

@@ -268,9 +268,11 @@ def adjust_logits(logits, history=None, repeat=None, frequency=None, presence=No
     ``history`` = (offsets (rows + 1) int32, tokens int32): for each token
     that occurs c times in the row's slice, l / ``repeat`` if l > 0 else l *
     ``repeat``, then minus ``frequency`` * c + ``presence`` (each (rows)
-    float32). ``bias`` = (offsets, tokens, float32 values) is added (a token
-    listed twice takes its last entry). ``mask`` (rows, words) int32: bit t %
-    32 of word t // 32 is 0 for a forbidden token, which becomes -inf.
+    float32). All three go by the same history: for a repetition over prompt
+    and output and the others over the output alone, call twice, in place.
+    ``bias`` = (offsets, tokens, float32 values) is added (a token listed
+    twice takes its last entry). ``mask`` (rows, words) int32: bit t % 32 of
+    word t // 32 is 0 for a forbidden token, which becomes -inf.
     Returns (out, argmax (rows) int32); ``out`` may be ``logits`` itself,
     ``argmax`` a tensor to fill, or False for none."""
     if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.get_device() < 0:

@@ -465,3 +465,30 @@ def test_many_small_weights_beside_a_large_one(sv, n_seq, rows, hd, tol):
     got = sv.KVPool(data, 8, hd, page).attend(batch_of(sv, [rows] * n_seq, [ln] * n_seq, table), q).double()
     value = 127 * float(np.float32(0.3 / 127))
     assert (got / value - 1).abs().max() < tol
+
+
+def test_penalties_over_two_histories(sv):
+    """Repetition over prompt and output, frequency and presence over the
+    output alone: two calls in place give the definition."""
+    import torch
+    rng = np.random.default_rng(97)
+    x = (3 * rng.standard_normal((1, 500))).astype(np.float32)
+    whole, out = rng.integers(0, 500, 200).astype(np.int32), rng.integers(0, 500, 60).astype(np.int32)
+    allowed = rng.random(500) < 0.7
+    words = np.packbits(np.concatenate([allowed, np.zeros(12, bool)])[None], axis=1, bitorder="little").view(np.int32)
+
+    def lists(t):
+        return dev(np.array([0, t.size], np.int32)), dev(t)
+
+    def one(v):
+        return torch.full((1,), v, device="cuda")
+
+    lg = dev(x)
+    sv.adjust_logits(lg, history=lists(whole), repeat=one(1.25), out=lg, argmax=False)
+    _, am = sv.adjust_logits(lg, history=lists(out), frequency=one(0.25), presence=one(0.5), mask=dev(words), out=lg)
+    want = ref.adjust(x[0], whole, 1.25, 0.0, 0.0, [], None)
+    want = ref.adjust(want, out, 1.0, 0.25, 0.5, [], allowed)
+    got = lg.cpu().numpy()[0]
+    f = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), f) and np.abs(got[f] - want[f]).max() <= 1e-6 * (2 * np.abs(x).max() + 20)
+    assert am.item() == int(np.argmax(got))
